@@ -1,0 +1,373 @@
+"""The 8-bit paged KV cache and its attention, as they are measured.
+
+Three operators, each in its plain form (elementary torch operations in 32 bits)
+and as a user calls it (``own``):
+
+* write: rows of K and V are quantised into the paged 8-bit arenas. A row of one
+  token and KV head shares one power-of-two scale 2^e: e is the smallest integer
+  (at least -100) with max|x| <= M * 2^e, M the largest code (448 for E4M3, 127
+  for INT8); code = nearest(x * 2^-e), ties to even.
+* read: the rows of given slots come back as code * 2^e.
+* attention: causal attention of each sequence's new rows over its cached
+  positions through a block table, G query heads per KV head; with a window w a
+  query at position p sees j <= p with j > p - w or j < sinks.
+
+Arenas: codes [blocks, layers, block_size, heads * head_dim], exponents
+[blocks, layers, heads, block_size] int8, one pair each for K and V.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+LAYERS = 2      # the arenas hold two layers, the calls address the second
+LAYER = 1
+E_MIN = -100
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def listed():
+    write = {"op": "write", "hd": 128, "block": 16}
+    read = {"op": "read", "hd": 128, "block": 16}
+    attn = {"op": "attention", "hd": 128, "block": 16, "window": 0, "sinks": 0}
+    return [
+        # one decode step of one sequence: the smallest write
+        {**write, "name": "write 1 token", "tokens": 1, "kv_heads": 32, "format": "e4m3", "type": "fp32", "skip": 0.0},
+        # a step that holds whole prompts, 4096-wide fp32 rows as slices of a fused QKV buffer
+        {**write, "name": "write prompts fp32", "tokens": 10229, "kv_heads": 32, "format": "int8", "type": "fp32", "skip": 0.0},
+        # grouped heads of a 16-bit engine, a padded step (skipped rows), blocks that are not 16
+        {**write, "name": "write chunk bf16 hd64", "tokens": 4099, "kv_heads": 8, "hd": 64, "block": 24, "format": "e4m3", "type": "bf16", "skip": 0.1},
+        # a long sequence leaves the cache (moved to another GPU, or checked)
+        {**read, "name": "read 32768 rows fp32", "tokens": 32768, "kv_heads": 32, "format": "e4m3", "type": "fp32", "skip": 0.0},
+        # a short shared prefix
+        {**read, "name": "read prefix bf16 hd64", "tokens": 517, "kv_heads": 8, "hd": 64, "block": 8, "format": "int8", "type": "bf16", "skip": 0.1},
+        # one sequence decodes: latency
+        {**attn, "name": "decode 1 x 300", "prompts": "", "decodes": 1, "ctx_lo": 300, "ctx_hi": 300, "heads": 32, "kv_heads": 32, "format": "e4m3", "type": "fp32"},
+        # the decode workload of this repository on an 8-bit cache
+        {**attn, "name": "decode 64 x 512-4096", "prompts": "", "decodes": 64, "ctx_lo": 512, "ctx_hi": 4096, "heads": 32, "kv_heads": 32, "format": "e4m3", "type": "fp32"},
+        # its long-context decode, four query heads per KV head
+        {**attn, "name": "decode 4 x 32768 gqa", "prompts": "", "decodes": 4, "ctx_lo": 32768, "ctx_hi": 32768, "heads": 32, "kv_heads": 8, "format": "int8", "type": "bf16"},
+        # endless streams: window and sinks, eight query heads per KV head, ragged lengths
+        {**attn, "name": "decode 32 window", "prompts": "", "decodes": 32, "ctx_lo": 100, "ctx_hi": 16384, "heads": 64, "kv_heads": 8, "window": 1024, "sinks": 4, "format": "e4m3", "type": "bf16"},
+        # a late chunk of a long prompt: the largest
+        {**attn, "name": "chunk 4096 of 16384", "prompts": "4096/16384", "decodes": 0, "ctx_lo": 0, "ctx_hi": 0, "heads": 32, "kv_heads": 8, "format": "e4m3", "type": "bf16"},
+        # prompts beside decodes in one step, fp32 rows
+        {**attn, "name": "mixed 2 + 8 fp32", "prompts": "1537/1537,700/1900", "decodes": 8, "ctx_lo": 256, "ctx_hi": 8192, "heads": 32, "kv_heads": 32, "format": "int8", "type": "fp32"},
+        # a prompt under a window, head_dim 64
+        {**attn, "name": "prompt 8192 window hd64", "prompts": "8191/8191", "decodes": 0, "ctx_lo": 0, "ctx_hi": 0, "heads": 16, "kv_heads": 4, "hd": 64, "window": 1000, "sinks": 5, "format": "e4m3", "type": "bf16"},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    case = {"op": rng.choice(["write", "read", "attention", "attention", "attention"]), "hd": rng.choice([32, 64, 64, 128, 128, 128, 256]),
+            "block": rng.choice([8, 16, 16, 16, 24, 32, 64]), "format": rng.choice(["e4m3", "int8"]), "type": rng.choice(["fp32", "bf16", "bf16", "fp16"])}
+    if case["op"] != "attention":
+        heads = rng.choice([1, 2, 4, 8, 16, 32])
+        case.update(kv_heads=heads, tokens=_log(rng, 1, 32768 * 4096 // max(4096, heads * case["hd"])), skip=rng.choice([0.0, 0.05, 0.3]))
+        return case
+    group = rng.choice([1, 1, 2, 3, 4, 8])
+    kv = rng.choice([1, 2, 4, 8, 16, 32] if group == 1 else [1, 2, 4, 8])
+    window, sinks = rng.choice([(0, 0), (0, 0), (_log(rng, 16, 4096), rng.choice([0, 1, 4, 17]))])
+    case.update(heads=kv * group, kv_heads=kv, window=window, sinks=sinks, prompts="", decodes=0, ctx_lo=0, ctx_hi=0)
+    kind = rng.choice(["decode", "decode", "chunk", "mixed"])
+    wide = kv * case["hd"] / 4096  # of a cached position, against the 32 x 128 of the largest cases
+    if kind in ("decode", "mixed"):
+        seqs = _log(rng, 1, 64)
+        hi = _log(rng, 1, min(32768, int(64 * 4096 / seqs / max(wide, 0.25))))
+        case.update(decodes=seqs, ctx_lo=rng.randint(1, hi), ctx_hi=hi)
+    if kind in ("chunk", "mixed"):
+        several = rng.randint(1, 3)
+        top = int(min(3500, math.sqrt(4096 * 16384 * 4 / case["heads"] / several)))
+        parts = []
+        for _ in range(several):
+            new = _log(rng, 2, top)
+            parts.append("%d/%d" % (new, new + rng.choice([0, 0, rng.randint(1, top)])))
+        case["prompts"] = ",".join(parts)
+    return case
+
+
+def _plan(case):
+    """(new rows, context) of each sequence of an attention case, prompts first; decode contexts spread evenly over their range."""
+    seqs = [tuple(int(v) for v in p.split("/")) for p in case["prompts"].split(",") if p]
+    n, lo, hi = case["decodes"], case["ctx_lo"], case["ctx_hi"]
+    return seqs + [(1, lo + (hi - lo) * ((i * 7) % n) // max(1, n - 1 or 1)) for i in range(n)]
+
+
+def _visible(case):
+    """Visible (row, key) pairs and cached positions that some row sees, over all sequences."""
+    w, sinks, pairs, seen = case["window"], case["sinks"], 0, 0
+    for new, ctx in _plan(case):
+        p = np.arange(ctx - new, ctx, dtype=np.int64)
+        first = np.maximum(0, p - w + 1) if w else np.zeros_like(p)
+        pairs += int((p - first + 1 + np.minimum(sinks if w else 0, first)).sum())
+        seen += int(ctx - first[0] + min(sinks if w else 0, first[0]))
+    return pairs, seen
+
+
+def work(case):
+    size = 4 if case["type"] == "fp32" else 2
+    if case["op"] != "attention":
+        rows = round(case["tokens"] * (1 - case["skip"])) * case["kv_heads"]
+        return {"bytes": 2 * rows * (case["hd"] * (size + 1) + 1) + 4 * case["tokens"], "flops": 0}
+    pairs, seen = _visible(case)
+    new = sum(n for n, _ in _plan(case))
+    return {"bytes": 2 * seen * case["kv_heads"] * (case["hd"] + 1) + 2 * new * case["heads"] * case["hd"] * size,
+            "flops": 4 * pairs * case["heads"] * case["hd"]}
+
+
+def _exponent(a, top):
+    """The smallest integer e >= E_MIN with a <= top * 2^e, for a tensor of maxima."""
+    m, x = torch.frexp(a)            # a = m * 2^x, m in [0.5, 1)
+    tm, tx = math.frexp(top)
+    e = x - tx + (m > tm).to(x.dtype)
+    return torch.where(a > 0, e, torch.full_like(e, E_MIN)).clamp(min=E_MIN)
+
+
+def _quantise(x, fmt):
+    """codes (as bytes) and exponents of rows x [..., hd]."""
+    x = x.float()
+    e = _exponent(x.abs().amax(-1), 448.0 if fmt == "e4m3" else 127.0)
+    y = torch.ldexp(x, -e.unsqueeze(-1))
+    y = y.to(torch.float8_e4m3fn).view(torch.uint8) if fmt == "e4m3" else y.round().to(torch.int8).view(torch.uint8)
+    return y, e.to(torch.int8)
+
+
+def _values(codes, e, fmt):
+    """code * 2^e as 32-bit floats; codes (as bytes) [..., hd], e [...]."""
+    c = codes.view(torch.float8_e4m3fn if fmt == "e4m3" else torch.int8).float()
+    return torch.ldexp(c, e.unsqueeze(-1).int())
+
+
+def _rows(g, shape, kind):
+    """K/V-like rows: normal, with a spread of magnitudes over rows and a few outlying channels."""
+    x = torch.randn(shape, generator=g, device="cuda")
+    x *= torch.exp2(torch.randint(-2, 3, shape[:-1], generator=g, device="cuda").float()).unsqueeze(-1) if kind == "v" else 1.0
+    x[..., :: max(1, shape[-1] // 4)] *= 2.0
+    return x
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    kv, hd, B, fmt = case["kv_heads"], case["hd"], case["block"], case["format"]
+    t = TYPES[case["type"]]
+    s = dict(case)
+    if case["op"] == "attention":
+        plan = _plan(case)
+        need = [-(-c // B) for _, c in plan]
+    else:
+        need = [-(-case["tokens"] // B)]
+    blocks = sum(need) + 3
+    code = torch.float8_e4m3fn if fmt == "e4m3" else torch.int8
+    for n in "kv":  # arenas; a write starts from empty ones, the others read filled ones
+        codes = torch.zeros((blocks, LAYERS, B, kv * hd), dtype=torch.uint8, device="cuda")
+        exps = torch.full((blocks, LAYERS, kv, B), E_MIN, dtype=torch.int8, device="cuda")
+        if case["op"] != "write":
+            c, e = _quantise(_rows(g, (blocks, B, kv, hd), n), fmt)
+            codes[:, LAYER] = c.reshape(blocks, B, kv * hd)
+            exps[:, LAYER] = e.transpose(1, 2)
+        s[n + "_codes"], s[n + "_exps"] = codes.view(code), exps
+    order = torch.randperm(blocks, generator=g, device="cuda").int()
+    if case["op"] != "attention":
+        n = case["tokens"]
+        pos = torch.arange(n, device="cuda")
+        slots = (order[pos // B] * B + pos % B).int()
+        drop = torch.zeros(n, dtype=torch.bool, device="cuda")
+        drop[torch.randperm(n, generator=g, device="cuda")[: n - round(n * (1 - case["skip"]))]] = True
+        s["slots"] = torch.where(drop, -1, slots).int()
+        if case["op"] == "write":  # K and V as the engine has them: slices of one fused buffer
+            fused = torch.cat([_rows(g, (n, kv, hd), c).reshape(n, kv * hd) for c in "qkv"], 1).to(t)
+            s["key"], s["value"] = fused[:, kv * hd : 2 * kv * hd], fused[:, 2 * kv * hd :]
+        else:
+            s["key"], s["value"] = (torch.zeros((n, kv * hd), dtype=t, device="cuda") for _ in "kv")
+        return s
+    tables = torch.zeros((len(plan), max(need)), dtype=torch.int32, device="cuda")
+    at = 0
+    for i, b in enumerate(need):
+        tables[i, :b] = order[at : at + b]
+        at += b
+    new, ctx = [n for n, _ in plan], [c for _, c in plan]
+    s["tables"] = tables
+    s["cu"] = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32, device="cuda")
+    s["ctx"] = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    s["max_new"], s["max_ctx"] = max(new), max(ctx)
+    s["several"] = sum(n > 1 for n in new)  # sequences of several rows come first
+    s["last"] = sum(n for n in new if n > 1)  # and this many rows are theirs
+    s["max_ctx_one"] = max([c for n, c in plan if n == 1], default=0)
+    s["max_ctx_several"] = max([c for n, c in plan if n > 1], default=0)
+    s["query"] = torch.randn((sum(new), case["heads"] * hd), generator=g, device="cuda").to(t)
+    s["out"] = torch.zeros_like(s["query"])
+    return s
+
+
+def _attend(s, lo, hi, max_new, max_ctx, row_lo, row_hi):
+    """Plain attention of sequences lo..hi, padded to their longest, into rows row_lo..row_hi."""
+    if hi == lo:
+        return
+    kv, hd, B, fmt, H = s["kv_heads"], s["hd"], s["block"], s["format"], s["heads"]
+    S, G = hi - lo, H // kv
+    ctx, start = s["ctx"][lo:hi].long(), s["cu"][lo:hi].long()
+    new = s["cu"][lo + 1 : hi + 1].long() - start
+    nb = -(-max_ctx // B)
+    table = s["tables"][lo:hi, :nb].long()
+    k, v = (_values(s[n + "_codes"].view(torch.uint8)[table, LAYER].reshape(S, nb * B, kv, hd),
+                    s[n + "_exps"][table, LAYER].transpose(2, 3).reshape(S, nb * B, kv), fmt).transpose(1, 2) for n in "kv")
+    i = torch.arange(max_new, device="cuda")
+    rows = (start[:, None] + torch.minimum(i[None], new[:, None] - 1)).clamp(min=0)
+    q = s["query"][rows].float().reshape(S, max_new, kv, G, hd).permute(0, 2, 3, 1, 4).reshape(S, kv, G * max_new, hd)
+    scores = torch.matmul(q, k.transpose(2, 3)) * (1.0 / math.sqrt(hd))
+    p = (ctx - new)[:, None, None] + i[None, :, None]
+    j = torch.arange(nb * B, device="cuda")[None, None]
+    seen = j <= p
+    if s["window"]:
+        seen &= (j > p - s["window"]) | (j < s["sinks"])
+    scores = scores.reshape(S, kv, G, max_new, nb * B).masked_fill_(~seen[:, None, None], -math.inf)
+    scores -= scores.amax(-1, keepdim=True)
+    scores.exp_()
+    total = scores.sum(-1)
+    o = torch.matmul(scores.reshape(S, kv, G * max_new, nb * B), v).reshape(S, kv, G, max_new, hd) / total.unsqueeze(-1)
+    o = o.permute(0, 3, 1, 2, 4).reshape(S * max_new, H * hd)
+    there = (i[None] < new[:, None]).reshape(-1).nonzero().squeeze(1)
+    s["out"][row_lo:row_hi] = o[there].to(s["out"].dtype)
+
+
+def _plain(s):
+    kv, hd, B, fmt = s["kv_heads"], s["hd"], s["block"], s["format"]
+    if s["op"] == "attention":
+        m = s["several"]
+        _attend(s, 0, m, s["max_new"], s["max_ctx_several"], 0, s["last"])
+        _attend(s, m, len(s["ctx"]), 1, s["max_ctx_one"], s["last"], len(s["out"]))
+        return s["out"]
+    rows = (s["slots"] >= 0).nonzero().squeeze(1)
+    slots = s["slots"][rows].long()
+    block, at = slots // B, slots % B
+    if s["op"] == "write":
+        for n, x in (("k", s["key"]), ("v", s["value"])):
+            c, e = _quantise(x[rows].reshape(-1, kv, hd), fmt)
+            s[n + "_codes"].view(torch.uint8)[block, LAYER, at] = c.reshape(-1, kv * hd)
+            s[n + "_exps"][block, LAYER, :, at] = e
+        return {n: s[n] for n in ("k_codes", "v_codes", "k_exps", "v_exps")}
+    for n, x in (("k", s["key"]), ("v", s["value"])):
+        c = s[n + "_codes"].view(torch.uint8)[block, LAYER, at].reshape(-1, kv, hd)
+        x[rows] = _values(c, s[n + "_exps"][block, LAYER, :, at], fmt).reshape(-1, kv * hd).to(x.dtype)
+    return {"key": s["key"], "value": s["value"]}
+
+
+def _nvllm():
+    import sys
+    from pathlib import Path
+    package = str(Path.cwd() / "nano-vllm-cpp26_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import nvllm
+    return nvllm
+
+
+def _own(s):
+    nvllm = _nvllm()
+    if "arena" not in s:  # the arena's handle and the workspace: made once and kept, as an engine does
+        layout = nvllm.KVLayout(len(s["k_codes"]), LAYERS, s["block"], s["kv_heads"], s["hd"])
+        s["arena"] = nvllm.KV8Arena(layout, s["k_codes"], s["v_codes"], s["k_exps"], s["v_exps"])
+        if s["op"] == "attention":
+            s["workspace"] = nvllm.kv8_alloc_workspace(len(s["ctx"]), s["max_new"], s["max_ctx"], s["heads"], layout)
+    if s["op"] == "write":
+        nvllm.kv8_write(s["key"], s["value"], s["arena"], s["slots"], LAYER)
+        return {n: s[n] for n in ("k_codes", "v_codes", "k_exps", "v_exps")}
+    if s["op"] == "read":
+        nvllm.kv8_read(s["key"], s["value"], s["arena"], s["slots"], LAYER)
+        return {"key": s["key"], "value": s["value"]}
+    nvllm.kv8_attention(s["out"], s["query"], s["arena"], s["tables"], s["cu"], s["ctx"], s["max_new"], s["max_ctx"], LAYER,
+                        num_heads=s["heads"], window=s["window"], sinks=s["sinks"], workspace=s["workspace"])
+    return s["out"]
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def _code_values(fmt):
+    """The value of each of the 256 codes, from the format's definition; codes that are not numbers are NaN."""
+    if fmt == "int8":
+        return np.array([b - 256 if b > 127 else b for b in range(256)], np.float64)
+    v = []
+    for b in range(256):
+        x, m = (b >> 3) & 15, b & 7
+        a = math.nan if x == 15 and m == 7 else m * 2.0 ** -9 if x == 0 else (8 + m) * 2.0 ** (x - 10)
+        v.append(-a if b & 128 else a)
+    return np.array(v, np.float64)
+
+
+def _nearest(y, fmt):
+    """Rounds 64-bit values to the nearest code's value, ties to the even code."""
+    if fmt == "int8":
+        return torch.round(y)
+    grid = torch.from_numpy(_code_values(fmt)[:127].copy()).to(y.device)  # 0 .. 448, code = place
+    a = y.abs()
+    hi = torch.searchsorted(grid, a).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    up, down = grid[hi] - a, a - grid[lo]
+    take = torch.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+    return torch.copysign(grid[take], y)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    kv, hd, B, fmt = s["kv_heads"], s["hd"], s["block"], s["format"]
+    top = 448.0 if fmt == "e4m3" else 127.0
+    if case["op"] == "write":
+        kept = s["slots"] >= 0
+        at = s["slots"][kept].long()
+        out = {}
+        for n, x in (("k", s["key"]), ("v", s["value"])):
+            x = x[kept].double().reshape(-1, kv, hd)
+            a = x.abs().amax(-1)
+            e = torch.full_like(a, E_MIN)
+            e = torch.where(a > 0, torch.ceil(torch.log2(torch.clamp(a, min=1e-300) / top)), e)
+            e = torch.where(a > top * torch.exp2(e), e + 1, e)       # log2 may be an ulp off at the border
+            e = torch.where(a <= top * torch.exp2(e - 1), e - 1, e)
+            e = torch.clamp(e, min=E_MIN)
+            codes = torch.zeros((len(s["k_codes"]) * B, kv * hd), dtype=torch.float64, device="cuda")
+            exps = torch.full((len(s["k_codes"]) * B, kv), E_MIN, dtype=torch.int8, device="cuda")
+            codes[at] = _nearest(x * torch.exp2(-e).unsqueeze(-1), fmt).reshape(-1, kv * hd)
+            exps[at] = e.to(torch.int8)
+            full = torch.zeros((len(s["k_codes"]), LAYERS, B, kv * hd), dtype=torch.float64, device="cuda")
+            full[:, LAYER] = codes.reshape(-1, B, kv * hd)
+            fexp = torch.full((len(s["k_codes"]), LAYERS, kv, B), E_MIN, dtype=torch.int8, device="cuda")
+            fexp[:, LAYER] = exps.reshape(-1, B, kv).transpose(1, 2)
+            out[n + "_codes"], out[n + "_exps"] = (full if fmt == "e4m3" else full.to(torch.int8)), fexp
+        return out
+    table = torch.from_numpy(_code_values(fmt)).cuda()
+    k, v = ((table[s[n + "_codes"].view(torch.uint8)[:, LAYER].int()].reshape(-1, B, kv, hd)
+             * torch.exp2(s[n + "_exps"][:, LAYER].double()).transpose(1, 2).unsqueeze(-1)).reshape(-1, kv, hd) for n in "kv")
+    if case["op"] == "read":
+        there = (s["slots"] >= 0)[:, None, None]
+        at = s["slots"].clamp(min=0).long()
+        return {n: torch.where(there, x[at], 0.0).reshape(len(at), kv * hd) for n, x in (("key", k), ("value", v))}
+    pairs, _ = _visible(case)
+    if 4 * pairs * case["heads"] * hd > 4e12:
+        return None
+    G = case["heads"] // kv
+    out = torch.zeros(s["out"].shape, dtype=torch.float64, device="cuda")
+    at = 0
+    for i, (new, ctx) in enumerate(_plan(case)):
+        j = torch.arange(ctx, device="cuda")
+        slots = s["tables"][i].long()[j // B] * B + j % B
+        for first in range(0, new, 512):
+            n = min(512, new - first)
+            p = ctx - new + first + torch.arange(n, device="cuda")[:, None]
+            hidden = j[None] > p
+            if case["window"]:
+                hidden |= (j[None] <= p - case["window"]) & (j[None] >= case["sinks"])
+            for h in range(case["heads"]):
+                q = s["query"][at + first : at + first + n, h * hd : (h + 1) * hd].double()
+                z = (q @ k[slots, h // G].T) / math.sqrt(hd)
+                z[hidden] = -math.inf
+                out[at + first : at + first + n, h * hd : (h + 1) * hd] = torch.softmax(z, 1) @ v[slots, h // G]
+        at += new
+    return out
