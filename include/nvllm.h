@@ -1,8 +1,8 @@
 /*
  * nvllm — B200 (sm_100a) paged-KV write + paged attention for nano-vllm-cpp26.
  *
- * C ABI of libnvllm.so. All tensors are fp32 device pointers owned by the
- * caller; every call is asynchronous on the caller's CUDA stream (passed as
+ * C ABI of libnvllm.so. All tensors are device pointers owned by the caller, of
+ * fp32 except where a call takes an nvllm_dtype; every call is asynchronous on the caller's CUDA stream (passed as
  * void*, i.e. a cudaStream_t; NULL = legacy default stream) and allocates
  * nothing. Return value: NVLLM_OK or one of the NVLLM_ERR_* codes below.
  *
@@ -159,6 +159,91 @@ int nvllm_paged_attention_head_split(const nvllm_head_split* hs, const float* qu
                                      int32_t num_seqs, int32_t max_context_len, int32_t layer,
                                      float scale, void* workspace, size_t workspace_bytes,
                                      const nvllm_kv_layout* layout, void* stream);
+
+/* ---- 8-bit paged KV cache --------------------------------------------------
+ *
+ * The same paged geometry with one byte per value instead of four, for rows of
+ * fp32, bf16 or fp16 and grouped heads. A cached row of one (token, KV head) is
+ * head_dim codes and one exponent e: value = code * 2^e. e is the smallest
+ * integer >= -100 with max|x| <= M * 2^e, M the largest code (448 for E4M3,
+ * 127 for INT8), and code = x * 2^-e rounded to the nearest code, ties to even.
+ * With the scale a power of two, x * 2^-e is exact (codes are reproducible bit
+ * for bit on any machine) and a cached value has at most 8 significant bits, so
+ * that it is read back exactly into fp32 and bf16 and enters the tensor cores
+ * as a bf16 operand without a rounding. The reference has no such cache; its
+ * fp32 arena is include/nano_vllm/kv_cache.hpp:30-33.
+ */
+enum nvllm_dtype { NVLLM_DTYPE_FP32 = 0, NVLLM_DTYPE_BF16 = 1, NVLLM_DTYPE_FP16 = 2 };
+enum nvllm_kv8_format {
+    NVLLM_KV8_E4M3 = 0, /* 8-bit float: relative error <= 2^-4 of each value */
+    NVLLM_KV8_INT8 = 1  /* 8-bit integer: absolute error <= max|x| / 127 of the row */
+};
+
+/* Arenas on the device, owned by the caller. Codes: [num_blocks, num_layers,
+ * block_size, num_heads * head_dim] bytes, like the fp32 arena; 16-byte aligned.
+ * Exponents: [num_blocks, num_layers, num_heads, block_size] int8 (the
+ * positions of a block adjacent, as the attention reads them). num_heads of the
+ * layout counts KV heads. A call reads no slot beyond a sequence's context, so
+ * the arenas need no clearing. */
+typedef struct nvllm_kv8_arena {
+    void* k_codes;
+    void* v_codes;
+    int8_t* k_exps;
+    int8_t* v_exps;
+    int32_t format; /* nvllm_kv8_format */
+} nvllm_kv8_arena;
+
+/* Quantises num_tokens rows of key and value (dtype: nvllm_dtype; row t starts
+ * at element t * key_stride / t * value_stride, strides >= num_heads * head_dim,
+ * so that slices of a fused QKV buffer need no copy) into arena rows
+ * (slot_mapping[t] / B, layer, slot_mapping[t] % B). NaN is stored as 0, and
+ * values are clamped to +-M * 2^119 (infinities included). A negative slot
+ * skips the token; a slot beyond the arena is skipped and raises
+ * NVLLM_ERR_BOUNDS in nvllm_get_last_error(). Slots must be distinct: where two
+ * rows of a call share one, what that slot holds is unspecified. */
+int nvllm_kv8_write(const void* key, const void* value, int32_t dtype, int64_t key_stride,
+                    int64_t value_stride, const nvllm_kv8_arena* arena,
+                    const int32_t* slot_mapping, int64_t num_tokens, int32_t layer,
+                    const nvllm_kv_layout* layout, void* stream);
+
+/* Reads rows back: key / value row t = the values of slot slot_mapping[t],
+ * exact in fp32 and bf16, rounded to nearest in fp16 (beyond its range:
+ * infinity). Rows of negative slots are left as they were, as are those of slots
+ * beyond the arena, which raise NVLLM_ERR_BOUNDS. */
+int nvllm_kv8_read(void* key, void* value, int32_t dtype, int64_t key_stride,
+                   int64_t value_stride, const nvllm_kv8_arena* arena,
+                   const int32_t* slot_mapping, int64_t num_tokens, int32_t layer,
+                   const nvllm_kv_layout* layout, void* stream);
+
+/* Bytes of device workspace nvllm_kv8_attention needs for a batch of at most
+ * num_seqs sequences with these maxima and num_query_heads query heads. 0 for
+ * arguments that the call refuses. */
+size_t nvllm_kv8_attention_workspace_size(int32_t num_seqs, int32_t max_query_len,
+                                          int32_t max_context_len, int32_t num_query_heads,
+                                          const nvllm_kv_layout* layout);
+
+/* Causal attention of each sequence's new rows (one, a chunk, or a whole
+ * prompt; mixed batches as in nvllm_paged_attention, with the same metadata)
+ * over one layer of the 8-bit cache. query and out hold num_query_heads heads
+ * of head_dim per row (dtype: nvllm_dtype; row strides in elements, multiples
+ * of 16 bytes); query head h reads KV head h / (num_query_heads / num_heads).
+ * window > 0: the row at position p sees the positions j <= p with
+ * j > p - window or j < sinks (a sliding window of `window` positions, itself
+ * included, and the sequence's first `sinks` positions); window 0: all j <= p
+ * (sinks is then not used). Positions whose block id lies outside the arena
+ * count as zero rows and raise NVLLM_ERR_BOUNDS; a sequence whose metadata
+ * contradicts the maxima is skipped (its rows stay as they were) and raises
+ * NVLLM_ERR_INVALID in nvllm_get_last_error. Rows that belong to no sequence
+ * are not touched. The workspace (256-byte aligned) is overwritten by each
+ * call: calls that may overlap on the GPU need one each. */
+int nvllm_kv8_attention(void* out, int64_t out_stride, const void* query, int64_t query_stride,
+                        int32_t dtype, const nvllm_kv8_arena* arena,
+                        const int32_t* block_tables, int32_t max_blocks_per_seq,
+                        const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                        int32_t num_seqs, int32_t max_query_len, int32_t max_context_len,
+                        int32_t num_query_heads, int32_t layer, float scale, int32_t window,
+                        int32_t sinks, void* workspace, size_t workspace_bytes,
+                        const nvllm_kv_layout* layout, void* stream);
 
 /* Synchronizes the stream, then returns (and clears) the device status word
  * of the current device that the kernels set on skipped out-of-range accesses,

@@ -5,9 +5,14 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include "../../include/nvllm.h"
 #include "common.cuh"
 
 namespace nvllm {
+
+// Checks of a layout (NVLLM_OK or the status to return) and its strides.
+int validate_layout(const nvllm_kv_layout* lay);
+ArenaGeom make_geom(const nvllm_kv_layout* lay);
 
 // Work items produced by the plan kernel.
 //   decode item  (seq, split):  positions [split*P, min((split+1)*P, ctx))

@@ -25,6 +25,8 @@ bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u
 
 bool head_dim_supported(int32_t hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
+}  // namespace
+
 int validate_layout(const nvllm_kv_layout* lay) {
     if (lay == nullptr) return NVLLM_ERR_INVALID;
     if (lay->num_blocks <= 0 || lay->num_layers <= 0 || lay->block_size <= 0 ||
@@ -49,8 +51,6 @@ ArenaGeom make_geom(const nvllm_kv_layout* lay) {
     g.head_dim = lay->head_dim;
     return g;
 }
-
-}  // namespace
 
 WorkspaceLayout workspace_layout(int32_t num_seqs, int32_t max_query_len, int32_t max_context_len,
                                  int32_t num_heads, int32_t head_dim) {

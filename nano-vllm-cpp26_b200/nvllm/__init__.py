@@ -9,6 +9,9 @@ Reference correspondence (nano-vllm-cpp26):
   * :func:`reshape_and_cache`  -> the write_kv loop, src/model.cpp:188-202
   * :func:`paged_attention`    -> step 3d of forward_batch, src/model.cpp:204-260
   * :class:`KVLayout`          -> KVCacheConfig, include/nano_vllm/kv_cache.hpp:18-28
+
+The 8-bit cache (:class:`KV8Arena`, :func:`kv8_write`, :func:`kv8_read`,
+:func:`kv8_attention`) is in kv8.py.
 """
 from __future__ import annotations
 
@@ -223,3 +226,7 @@ def paged_attention_head_split(hs: HeadSplit, query, k_arena, v_arena, block_tab
     if check:
         _check(st, "nvllm_paged_attention_head_split")
     return st
+
+
+from .kv8 import (KV8_E4M3, KV8_INT8, KV8Arena, kv8_alloc_workspace, kv8_attention,  # noqa: E402
+                  kv8_read, kv8_workspace_size, kv8_write)

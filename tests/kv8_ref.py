@@ -1,0 +1,105 @@
+"""The 8-bit paged KV cache in plain numpy, 64 bits: codes, values, attention,
+and how far a kernel's output may be from it.
+
+Quantisation: with M = 448 (E4M3) or 127 (INT8), x' = 0 for NaN else x clamped to
++-M 2^119, e the smallest integer >= -100 with max|x'| <= M 2^e, code = x' 2^-e
+rounded to the nearest code, ties to even.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+
+E_MIN = -100
+MAX = {"e4m3": 448.0, "int8": 127.0}
+
+
+def e4m3_table() -> np.ndarray:
+    """Values of the 256 E4M3 bytes (the two NaN codes as NaN)."""
+    out = np.empty(256)
+    for b in range(256):
+        x, m = (b >> 3) & 15, b & 7
+        a = math.nan if (x, m) == (15, 7) else m * 2.0 ** -9 if x == 0 else (8 + m) * 2.0 ** (x - 10)
+        out[b] = -a if b & 128 else a
+    return out
+
+
+def code_values(codes: np.ndarray, fmt: str) -> np.ndarray:
+    """codes as bytes -> their values."""
+    return e4m3_table()[codes] if fmt == "e4m3" else codes.view(np.int8).astype(np.float64)
+
+
+def quantise(x: np.ndarray, fmt: str):
+    """Rows x [..., hd] (float64) -> (codes as bytes, exponents int8)."""
+    top = MAX[fmt]
+    x = np.where(np.isnan(x), 0.0, x)
+    x = np.clip(x, -top * 2.0 ** 119, top * 2.0 ** 119)
+    a = np.abs(x).max(-1)
+    e = np.full(a.shape, E_MIN)
+    for i, v in np.ndenumerate(a):
+        k = E_MIN
+        while v > top * 2.0 ** k:
+            k += 1
+        e[i] = k
+    y = x * 2.0 ** -e[..., None].astype(np.float64)
+    if fmt == "int8":
+        return np.rint(y).astype(np.int8).view(np.uint8), e.astype(np.int8)
+    grid = e4m3_table()[:127]
+    m = np.abs(y)
+    hi = np.clip(np.searchsorted(grid, m), 0, 126)
+    lo = np.maximum(hi - 1, 0)
+    up, down = grid[hi] - m, m - grid[lo]
+    code = np.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+    return (code + 128 * np.signbit(y)).astype(np.uint8), e.astype(np.int8)
+
+
+def dequantise(codes: np.ndarray, exps: np.ndarray, fmt: str) -> np.ndarray:
+    return code_values(codes, fmt) * 2.0 ** exps[..., None].astype(np.float64)
+
+
+def attention(q, k, v, first_pos: int, group: int, scale: float, window: int = 0, sinks: int = 0):
+    """q [rows, H, hd], k, v [ctx, Hkv, hd] (float64) -> (out, sum_j w_j |V_j|,
+    max_j scale sum_d |q_d K_jd|, visible keys), the last two per (row, head)."""
+    rows, H, hd = q.shape
+    ctx = k.shape[0]
+    kk, vv = np.repeat(k, group, 1), np.repeat(v, group, 1)
+    z = np.einsum("rhd,jhd->rhj", q, kk) * scale
+    p = first_pos + np.arange(rows)[:, None]
+    j = np.arange(ctx)[None]
+    seen = j <= p
+    if window:
+        seen &= (j > p - window) | (j < sinks)
+    z = np.where(seen[:, None], z, -np.inf)
+    z -= z.max(-1, keepdims=True)
+    w = np.exp(z)
+    w /= w.sum(-1, keepdims=True)
+    mag = np.einsum("rhd,jhd->rhj", np.abs(q), np.abs(kk)) * scale
+    mag = np.where(seen[:, None], mag, 0.0).max(-1)
+    n = np.broadcast_to(seen.sum(-1)[:, None], (rows, H))
+    return (np.einsum("rhj,jhd->rhd", w, vv), np.einsum("rhj,jhd->rhd", w, np.abs(vv)), mag, n)
+
+
+# Roundings, relative to the value: half a step of each type.
+HALF = {"fp32": 2.0 ** -24, "bf16": 2.0 ** -8, "fp16": 2.0 ** -11}
+# What the kernels may round a softmax weight to before the product with V: 24
+# bits for fp32 rows, one bf16 for bf16 rows, two bf16 terms for fp16 rows.
+WEIGHT = {"fp32": 2.0 ** -24, "bf16": 2.0 ** -8, "fp16": 2.0 ** -16}
+# An fp16 result below 2^-14 is a multiple of 2^-24, so rounding to it is off by up
+# to 2^-25 whatever its size (an output is that small where the only value with a
+# weight that counts is 0); fp32 and bf16 steps go down to 2^-149 and 2^-133.
+SMALLEST = {"fp32": 2.0 ** -150, "bf16": 2.0 ** -134, "fp16": 2.0 ** -25}
+
+
+def tolerance(out, vabs, mag, n, hd: int, dtype: str) -> np.ndarray:
+    """How far an output may be from the exact one.
+
+    A score is a sum of hd products in 32 bits: its error is at most
+    ds = (hd + 8) 2^-23 mag (a truncating adder loses a whole step per addition;
+    the 8 for the scale, the logarithm's base and the exponent's argument), plus
+    2^-22 for the exponential. A weight then is off by exp(ds) - 1, the sum of
+    the weights by as much plus its n additions, and the sum with V by n
+    additions more; the weight's own rounding and the output's come on top."""
+    ds = (hd + 8) * 2.0 ** -23 * mag + 2.0 ** -22
+    rel = 2 * np.expm1(ds) + (2 * n + 16) * 2.0 ** -23 + WEIGHT[dtype]
+    return rel[..., None] * vabs + HALF[dtype] * np.abs(out) + SMALLEST[dtype]
