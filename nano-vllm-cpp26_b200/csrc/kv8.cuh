@@ -62,6 +62,61 @@ struct Kv8AttnParams {
     float qk_scale_log2;  // softmax scale * log2(e)
 };
 
+// ---- work list ---------------------------------------------------------------
+// A query tile is `tile_rows` consecutive packed rows of one sequence and KV head:
+// packed row r is token r / group, query head kv_head * group + r % group, so that
+// the heads of a group share what is read. Its visible positions, in chunks of
+// `chunk` positions aligned to multiples of it, form a list: first the chunks
+// that hold sink positions, then those from the window's start to the tile's
+// last position. An item is a run of one tile's list; a tile that one item covers
+// writes its rows, the parts of others leave (m, l, acc) partials to be merged.
+struct Kv8Item {
+    int32_t seq;
+    int32_t row0;    // first packed row
+    int32_t c0, c1;  // the run of the tile's list
+    int32_t nsink;   // chunks of sinks at its start
+    int32_t lo;      // chunk of its first entry after them
+    int32_t slot;    // partial slot (times KV heads, plus the head), < 0: whole tile
+    int32_t pad;
+};
+struct Kv8Merge {
+    int32_t seq;
+    int32_t row0;
+    int32_t slot;   // of the first part
+    int32_t parts;
+};
+struct Kv8Counters {
+    int32_t next;    // cursor over items x KV heads
+    int32_t items;
+    int32_t merges;
+    int32_t slots;
+};
+struct Kv8Work {
+    Kv8Counters* counters;
+    Kv8Item* items;
+    Kv8Merge* merges;
+    float* acc;    // [slot][tile_rows][head_dim], weights relative to 2^m
+    float2* ml;    // [slot][tile_rows] (m, l)
+    int32_t tile_rows;
+    int32_t chunk;
+    int32_t min_run;   // shortest run (chunks) a tile is cut into
+    int32_t target;    // runs to aim for, over all KV heads
+    int32_t merge_grid;  // CTAs of the merge, 0: no tile is ever cut
+};
+
+// Carves the workspace for a work list whose tile_rows, chunk, min_run and target
+// are set (base may be NULL to learn the size, returned in bytes).
+size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_t max_query_len,
+                       int32_t max_context_len, int32_t group, const ArenaGeom& g);
+cudaError_t launch_kv8_plan(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t stream);
+cudaError_t launch_kv8_merge(const Kv8AttnParams& p, const Kv8Work& w, int32_t dtype,
+                             cudaStream_t stream);
+
+// Position of entry c of a tile's list, in chunks.
+__device__ __forceinline__ int kv8_chunk(const Kv8Item& it, int c) {
+    return c < it.nsink ? c : it.lo + c - it.nsink;
+}
+
 // True when the sequence's metadata agree with the call's bounds.
 __device__ __forceinline__ bool kv8_metadata_ok(const Kv8AttnParams& p, int q0, int qlen, int ctx) {
     return q0 >= 0 && qlen >= 0 && qlen <= ctx && qlen <= p.max_query_len &&

@@ -1,0 +1,235 @@
+// Work list of the 8-bit cache's attention, and the merge of cut tiles.
+//
+// The lengths live on the device, so one CTA builds the list: it counts the chunks
+// of every tile, W over all KV heads, and cuts tiles into runs of at most
+//   L = max(min_run, ceil(W / target)) chunks,
+// as equal as they come, so that a few long sequences fill the GPU as well as many
+// short ones. A tile of n > L chunks has ceil(n / L) <= 2 n / L parts, so there are
+// at most 2 target partial slots over all heads, whatever the batch.
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace nvllm {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
+
+// One sequence's rows and tiles; rows < 0: metadata that contradict the bounds.
+struct Kv8Seq {
+    int first_pos;  // position of its first new row
+    int rows;       // packed rows
+    int ntiles;
+};
+
+__device__ __forceinline__ Kv8Seq load_seq(const Kv8AttnParams& p, const Kv8Work& w, int s) {
+    const int q0 = p.cu_seqlens_q[s];
+    const int qlen = p.cu_seqlens_q[s + 1] - q0;
+    const int ctx = p.context_lens[s];
+    if (!kv8_metadata_ok(p, q0, qlen, ctx)) return {0, -1, 0};
+    const int rows = qlen * p.group;
+    return {ctx - qlen, rows, (rows + w.tile_rows - 1) / w.tile_rows};
+}
+
+// The list of tile t: chunks in all, of which sinks, and the first after them.
+struct Kv8List {
+    int n, nsink, lo;
+};
+__device__ __forceinline__ Kv8List tile_list(const Kv8AttnParams& p, const Kv8Work& w,
+                                             const Kv8Seq& q, int t) {
+    const int r0 = t * w.tile_rows;
+    const int r1 = min(r0 + w.tile_rows, q.rows) - 1;
+    const int p0 = q.first_pos + r0 / p.group;
+    const int p1 = q.first_pos + r1 / p.group;
+    const int first = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    const int lo = first / w.chunk;
+    const int nsink = min((min(p.sinks, first) + w.chunk - 1) / w.chunk, lo);
+    return {nsink + p1 / w.chunk + 1 - lo, nsink, lo};
+}
+
+// kWide: a warp per sequence, its lanes over the tiles; else a thread per sequence.
+template <bool kWide>
+__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnParams p, const Kv8Work w) {
+    __shared__ unsigned long long total;
+    __shared__ int n_items, n_slots, n_merges;
+    const int lane = threadIdx.x & 31;
+    const int me = kWide ? threadIdx.x >> 5 : threadIdx.x;
+    constexpr int kSeqs = kWide ? kPlanThreads / 32 : kPlanThreads;
+    constexpr int kStep = kWide ? 32 : 1;
+    const int t0 = kWide ? lane : 0;
+    if (threadIdx.x == 0) {
+        total = 0;
+        n_items = n_slots = n_merges = 0;
+    }
+    pdl_release();
+    pdl_wait();  // the metadata may come from the kernel before; the workspace is its
+    __syncthreads();
+    long long mine = 0;
+    for (int s = me; s < p.num_seqs; s += kSeqs) {
+        const Kv8Seq q = load_seq(p, w, s);
+        if (q.rows < 0 && t0 == 0) raise_status(kStatusMetadata);
+        for (int t = t0; t < q.ntiles; t += kStep) mine += tile_list(p, w, q, t).n;
+    }
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0 && mine) atomicAdd(&total, (unsigned long long)mine);
+    __syncthreads();
+    const long long all = (long long)total * p.a.num_heads;
+    const int run = int(max((long long)w.min_run, (all + w.target - 1) / w.target));
+    // the longest lists, those of a sequence's last tiles, go out first
+    for (int base = 0; base < p.num_seqs; base += kSeqs) {
+        const int s = base + me;
+        const Kv8Seq q = s < p.num_seqs ? load_seq(p, w, s) : Kv8Seq{0, 0, 0};
+        for (int i = 0;; i += kStep) {
+            const int t = q.ntiles - 1 - i - t0;
+            if (!__any_sync(0xffffffffu, t >= 0)) break;
+            const Kv8List l = t >= 0 ? tile_list(p, w, q, t) : Kv8List{0, 0, 0};
+            const int parts = t < 0 ? 0 : l.n > run ? (l.n + run - 1) / run : 1;
+            const int slots = parts > 1 ? parts : 0;
+            // this lane's places: an inclusive scan of both counts in one word
+            long long x = ((long long)(slots) << 32) | (unsigned)parts;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned cut = __ballot_sync(0xffffffffu, slots > 0);
+            int bi = 0, bs = 0, bm = 0;
+            if (lane == 31) {
+                bi = atomicAdd(&n_items, int(x & 0xffffffff));
+                if (cut) {
+                    bs = atomicAdd(&n_slots, int(x >> 32));
+                    bm = atomicAdd(&n_merges, __popc(cut));
+                }
+            }
+            bi = __shfl_sync(0xffffffffu, bi, 31) + int(x & 0xffffffff) - parts;
+            bs = __shfl_sync(0xffffffffu, bs, 31) + int(x >> 32) - slots;
+            bm = __shfl_sync(0xffffffffu, bm, 31) + __popc(cut & ((1u << lane) - 1));
+            for (int k = 0; k < parts; ++k) {
+                w.items[bi + k] = Kv8Item{s, t * w.tile_rows, int((long long)l.n * k / parts),
+                                          int((long long)l.n * (k + 1) / parts), l.nsink, l.lo,
+                                          parts > 1 ? bs + k : -1, 0};
+            }
+            if (slots > 0) w.merges[bm] = Kv8Merge{s, t * w.tile_rows, bs, parts};
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *w.counters = Kv8Counters{0, n_items, n_merges, n_slots};
+}
+
+// out = sum_k acc_k 2^(m_k - M) / sum_k l_k 2^(m_k - M), M = max_k m_k: a warp per
+// (cut tile, KV head, row), parts in order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p, const Kv8Work w) {
+    constexpr int PER = HD / 32;
+    pdl_release();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int H = p.a.num_heads;
+    const long long total = (long long)w.counters->merges * H * w.tile_rows;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += gridDim.x * 8ll) {
+        const int r = int(i % w.tile_rows);
+        const int h = int(i / w.tile_rows % H);
+        const Kv8Merge m = w.merges[i / w.tile_rows / H];
+        const int q0 = p.cu_seqlens_q[m.seq];
+        const int row = m.row0 + r;
+        if (row >= (p.cu_seqlens_q[m.seq + 1] - q0) * p.group) continue;
+        const auto at = [&](int k) { return (int64_t(m.slot + k) * H + h) * w.tile_rows + r; };
+        float M = -INFINITY;
+        for (int k = lane; k < m.parts; k += 32) M = fmaxf(M, __ldcg(&w.ml[at(k)].x));
+        M = warp_max_xor(M, 32);
+        float L = 0.f, o[PER];
+#pragma unroll
+        for (int d = 0; d < PER; ++d) o[d] = 0.f;
+        // a part in which the row sees nothing has m = -inf, l = 0
+        for (int k = 0; k < m.parts; k += 4) {
+            float2 ml[4];
+            float a[4][PER];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (k + u < m.parts) {
+                    ml[u] = __ldcg(&w.ml[at(k + u)]);
+#pragma unroll
+                    for (int d = 0; d < PER; ++d) a[u][d] = __ldcg(w.acc + at(k + u) * HD + d * 32 + lane);
+                } else {
+                    ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                    for (int d = 0; d < PER; ++d) a[u][d] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float f = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - M);
+                L = fmaf(ml[u].y, f, L);
+#pragma unroll
+                for (int d = 0; d < PER; ++d) o[d] = fmaf(a[u][d], f, o[d]);
+            }
+        }
+        const float inv = 1.0f / L;
+        T* dst = static_cast<T*>(p.out) + int64_t(q0 + row / p.group) * p.out_stride +
+                 int64_t(h * p.group + row % p.group) * HD;
+#pragma unroll
+        for (int d = 0; d < PER; ++d) dst[d * 32 + lane] = from_float<T>(o[d] * inv);
+    }
+}
+
+template <typename T>
+cudaError_t launch_merge_type(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
+    const dim3 grid(unsigned(w.merge_grid)), block(256);
+    switch (p.a.head_dim) {
+        case 32: return launch_programmatic(kv8_merge_kernel<T, 32>, grid, block, 0, st, p, w);
+        case 64: return launch_programmatic(kv8_merge_kernel<T, 64>, grid, block, 0, st, p, w);
+        case 128: return launch_programmatic(kv8_merge_kernel<T, 128>, grid, block, 0, st, p, w);
+        case 256: return launch_programmatic(kv8_merge_kernel<T, 256>, grid, block, 0, st, p, w);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_t max_query_len,
+                       int32_t max_context_len, int32_t group, const ArenaGeom& g) {
+    const int64_t tiles = (int64_t(max_query_len) * group + w.tile_rows - 1) / w.tile_rows;
+    const int64_t units = int64_t(num_seqs) * tiles;
+    // most chunks of one tile: two more than the positions, for the sinks' and the
+    // window's ragged ends
+    const int64_t chunks = (int64_t(max_context_len) + w.chunk - 1) / w.chunk + 2;
+    const bool cut = chunks > w.min_run;
+    const int64_t parts = cut ? (chunks + w.min_run - 1) / w.min_run : 1;
+    const int64_t slots = cut ? std::min<int64_t>(2 * int64_t(w.target) / g.num_heads + 1, units * parts) : 0;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        unsigned char* at = base + off;
+        off = align_up(off + bytes);
+        return at;
+    };
+    w.counters = reinterpret_cast<Kv8Counters*>(take(sizeof(Kv8Counters)));
+    w.items = reinterpret_cast<Kv8Item*>(take(size_t(units + slots) * sizeof(Kv8Item)));
+    w.merges = reinterpret_cast<Kv8Merge*>(take(size_t(slots) * sizeof(Kv8Merge)));
+    w.ml = reinterpret_cast<float2*>(take(size_t(slots) * g.num_heads * w.tile_rows * sizeof(float2)));
+    w.acc = reinterpret_cast<float*>(take(size_t(slots) * g.num_heads * w.tile_rows * g.head_dim * sizeof(float)));
+    const int64_t rows = std::min<int64_t>(units, slots) * g.num_heads * w.tile_rows;
+    w.merge_grid = int32_t(std::min<int64_t>((rows + 7) / 8, 148 * 4));
+    return off;
+}
+
+cudaError_t launch_kv8_plan(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t stream) {
+    const int64_t tiles = (int64_t(p.max_query_len) * p.group + w.tile_rows - 1) / w.tile_rows;
+    // a warp per sequence pays from a few tiles on; decode batches have one
+    return launch_programmatic(tiles > 4 ? kv8_plan_kernel<true> : kv8_plan_kernel<false>, dim3(1),
+                               dim3(kPlanThreads), 0, stream, p, w);
+}
+
+cudaError_t launch_kv8_merge(const Kv8AttnParams& p, const Kv8Work& w, int32_t dtype,
+                             cudaStream_t stream) {
+    switch (dtype) {
+        case NVLLM_DTYPE_FP32: return launch_merge_type<float>(p, w, stream);
+        case NVLLM_DTYPE_BF16: return launch_merge_type<__nv_bfloat16>(p, w, stream);
+        case NVLLM_DTYPE_FP16: return launch_merge_type<__half>(p, w, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace nvllm

@@ -8,6 +8,7 @@ rounded to the nearest code, ties to even.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import numpy as np
 
@@ -58,9 +59,17 @@ def dequantise(codes: np.ndarray, exps: np.ndarray, fmt: str) -> np.ndarray:
     return code_values(codes, fmt) * 2.0 ** exps[..., None].astype(np.float64)
 
 
+class Sizes(NamedTuple):
+    """What a row's error is measured by, per (row, head) but the first."""
+    vabs: np.ndarray  # sum_j w_j |V_j|, per dim
+    mag: np.ndarray   # max_j scale sum_d |q_d K_jd|
+    wide: np.ndarray  # max_j scale max_d|q_d| sum_d |K_jd|
+    top: np.ndarray   # max_j w_j max_d|V_jd|
+    n: np.ndarray     # visible positions
+
+
 def attention(q, k, v, first_pos: int, group: int, scale: float, window: int = 0, sinks: int = 0):
-    """q [rows, H, hd], k, v [ctx, Hkv, hd] (float64) -> (out, sum_j w_j |V_j|,
-    max_j scale sum_d |q_d K_jd|, visible keys), the last two per (row, head)."""
+    """q [rows, H, hd], k, v [ctx, Hkv, hd] (float64) -> (out, Sizes)."""
     rows, H, hd = q.shape
     ctx = k.shape[0]
     kk, vv = np.repeat(k, group, 1), np.repeat(v, group, 1)
@@ -76,30 +85,38 @@ def attention(q, k, v, first_pos: int, group: int, scale: float, window: int = 0
     w /= w.sum(-1, keepdims=True)
     mag = np.einsum("rhd,jhd->rhj", np.abs(q), np.abs(kk)) * scale
     mag = np.where(seen[:, None], mag, 0.0).max(-1)
+    wide = np.where(seen[:, None], np.abs(kk).sum(-1).T[None], 0.0).max(-1) * np.abs(q).max(-1) * scale
+    top = (w * np.abs(vv).max(-1).T[None]).max(-1)
     n = np.broadcast_to(seen.sum(-1)[:, None], (rows, H))
-    return (np.einsum("rhj,jhd->rhd", w, vv), np.einsum("rhj,jhd->rhd", w, np.abs(vv)), mag, n)
+    return np.einsum("rhj,jhd->rhd", w, vv), Sizes(np.einsum("rhj,jhd->rhd", w, np.abs(vv)), mag, wide, top, n)
 
 
 # Roundings, relative to the value: half a step of each type.
 HALF = {"fp32": 2.0 ** -24, "bf16": 2.0 ** -8, "fp16": 2.0 ** -11}
-# What the kernels may round a softmax weight to before the product with V: 24
-# bits for fp32 rows, one bf16 for bf16 rows, two bf16 terms for fp16 rows.
-WEIGHT = {"fp32": 2.0 ** -24, "bf16": 2.0 ** -8, "fp16": 2.0 ** -16}
+# What the kernels may round a softmax weight to before the product with V: two
+# fp16 terms for fp32 rows, one bf16 for bf16 rows, one fp16 for fp16 rows.
+WEIGHT = {"fp32": 2.0 ** -22, "bf16": 2.0 ** -8, "fp16": 2.0 ** -11}
 # An fp16 result below 2^-14 is a multiple of 2^-24, so rounding to it is off by up
 # to 2^-25 whatever its size (an output is that small where the only value with a
 # weight that counts is 0); fp32 and bf16 steps go down to 2^-149 and 2^-133.
 SMALLEST = {"fp32": 2.0 ** -150, "bf16": 2.0 ** -134, "fp16": 2.0 ** -25}
 
 
-def tolerance(out, vabs, mag, n, hd: int, dtype: str) -> np.ndarray:
+def tolerance(out, b: Sizes, hd: int, dtype: str) -> np.ndarray:
     """How far an output may be from the exact one.
 
     A score is a sum of hd products in 32 bits: its error is at most
-    ds = (hd + 8) 2^-23 mag (a truncating adder loses a whole step per addition;
-    the 8 for the scale, the logarithm's base and the exponent's argument), plus
-    2^-22 for the exponential. A weight then is off by exp(ds) - 1, the sum of
-    the weights by as much plus its n additions, and the sum with V by n
-    additions more; the weight's own rounding and the output's come on top."""
-    ds = (hd + 8) * 2.0 ** -23 * mag + 2.0 ** -22
-    rel = 2 * np.expm1(ds) + (2 * n + 16) * 2.0 ** -23 + WEIGHT[dtype]
-    return rel[..., None] * vabs + HALF[dtype] * np.abs(out) + SMALLEST[dtype]
+    (hd + 8) 2^-23 mag (a truncating adder loses a whole step per addition; the 8
+    for the scale, the logarithm's base and the exponent's argument). q enters as
+    fp16 terms of the row scaled to [1, 2): two leave at most 2^-23 of the row's
+    largest element, one (bf16 and fp16 rows) 2^-25 where an element is below
+    2^-14 of it: 2^-23 wide. The exponential adds 2^-22. A weight then is off by
+    exp(ds) - 1, the sum of the weights by as much plus its n additions, and the
+    sum with V by n additions more. A weight is rounded relative to itself, but to
+    no less than 2^-25 of the largest contribution w_j 2^(e_j) (an fp16 step
+    below 2^-14); times a code that is at most M 2^(e_j) < 2 max_d|V_jd|: n
+    2^-24 top in all. The output's own rounding comes on top."""
+    ds = (hd + 8) * 2.0 ** -23 * b.mag + 2.0 ** -23 * b.wide + 2.0 ** -22
+    rel = 2 * np.expm1(ds) + (2 * b.n + 16) * 2.0 ** -23 + WEIGHT[dtype]
+    return (rel[..., None] * b.vabs + (b.n * b.top)[..., None] * 2.0 ** -24 + HALF[dtype] * np.abs(out)
+            + SMALLEST[dtype])
