@@ -14,11 +14,15 @@
 //
 // Operands are fp16 terms: q' of fp32 rows as two (2^-23 of the row's largest
 // element), of bf16 and fp16 rows as one (exact up to 2^-25 of the largest); P of
-// fp32 rows as two terms (2^-23), of others as one (2^-12, less than the output's
-// own rounding). The two terms of a row are rows g and g + 8 of the same
-// 16-row tile, so that a tile of fp32 rows holds 8 rows and one MMA computes both
-// terms: at the few rows of a decode they cost nothing, and a lane adds its two
-// halves itself.
+// fp32 rows as two terms (2^-22), of others as one (2^-11, no more than the
+// output's own rounding).
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
+// positions and dims fill the MMA's 16 rows and the few query rows its 8 columns:
+// half the MMAs and accumulators of the other order. The two terms of an fp32 row
+// are columns 2r and 2r + 1, which one lane holds, and which it adds; with 4 rows
+// or fewer they cost nothing. P's pairs become the next product's operand by one
+// 8 x 8 transpose (movmatrix).
 //
 // What bounds a decode is the cache's bytes. A CTA of 4 warps takes runs of
 // chunks (kv8_plan.cu); a warp takes every fourth chunk of 16 positions and
@@ -26,9 +30,9 @@
 // pieces t, t + 4, .. of rows g and g + 8 (the MMA's order of the dims is
 // permuted to match, Q's fragments are stored that way); of V, the pieces of
 // dims g of rows 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes are paired across rows
-// as they are converted. No shared memory and no bank conflicts on the way; K of
-// the next chunk is in flight through the softmax and P V, V through Q K. The
-// warps' results are joined through shared memory at the end of a run.
+// as they are converted. No shared memory and no bank conflicts on the way; a
+// stage's registers are loaded again as soon as they are converted, STAGES chunks
+// ahead. The warps' results are joined through shared memory at the end of a run.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -51,9 +55,9 @@ struct Frag {
     static constexpr int VB = HD / 8 < 16 ? HD / 8 : 16;  // bytes of one V piece
     static constexpr int VP = HD / 8 / VB;                // V pieces of a lane per row
     static constexpr int KW = KB / 4;                     // words (MMA steps) per K piece
-    static constexpr int VW = VB / 4;                     // words (4 MMA tiles each) per V piece
+    static constexpr int VW = VB / 4;                     // words (2 MMA tiles each) per V piece
     static constexpr int KSTEPS = HD / 16;
-    static constexpr int NTILES = HD / 8;
+    static constexpr int MTILES = HD / 16;                // 16-dim tiles of O^T
 };
 
 template <int BYTES>
@@ -121,30 +125,43 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t h) {
     return pack_half(a - f.x, b - f.y);
 }
 
+// The 8 x 8 transpose of 16-bit values held as fragments.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // O of a row is rescaled only when the largest contribution grows by more than
 // this (log2): until then P <= 2^margin, and it cancels in acc / l.
 constexpr float kMargin = 4.0f;
 
-template <typename T, int HD, int MT>
+template <typename T, int HD, int NQ>
 struct Tile {
-    static constexpr int ROWS = MT * 16 / terms<T>();  // rows of a query tile
-    static constexpr int Q_WORDS = MT * (HD / 16) * 128;  // fragments of Q
+    static constexpr int ROWS = NQ * 8 / terms<T>();   // rows of a query tile
+    static constexpr int Q_WORDS = NQ * (HD / 16) * 64;  // fragments of Q
+    static constexpr bool Q_REGS = NQ * (HD / 16) <= 16; // held in registers
+    // chunks in flight per warp, as far as registers go
+    static constexpr int STAGES = HD == 256 || NQ > 2 || (HD == 128 && NQ > 1) ? 1 : 2;
     static constexpr int OROW = HD + 4;
     // the warps' results overlay Q's fragments
     static constexpr size_t JOIN = size_t(kWarps) * ROWS * (OROW + 2) * 4;
     static constexpr size_t SMEM = (Q_WORDS * 4 > JOIN ? Q_WORDS * 4 : JOIN) + ROWS * 4;
+    static constexpr int CTAS = HD * NQ >= 256 ? 2 : HD * NQ > 64 ? 3 : 4;
 };
 
-template <typename T, int kFormat, int HD, int MT, bool kB16>
-__global__ void __launch_bounds__(kWarps * 32, HD * MT >= 256 ? 2 : 3)
+template <typename T, int kFormat, int HD, int NQ, bool kB16>
+__global__ void __launch_bounds__(kWarps * 32, Tile<T, HD, NQ>::CTAS)
 kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     using F = Frag<HD>;
-    using S = Tile<T, HD, MT>;
+    using S = Tile<T, HD, NQ>;
     constexpr int NT = terms<T>();
-    constexpr int RL = NT == 2 ? 1 : 2;  // rows of a lane per 16-row tile
+    constexpr int RL = NT == 2 ? 1 : 2;    // rows of a lane per 8 columns
+    constexpr int OL = NT == 2 ? 2 : 4;    // sums of a lane per 16 x 8 tile of O^T
+    constexpr int ST = S::STAGES;
     extern __shared__ __align__(16) unsigned char smem[];
     uint32_t* sQ = reinterpret_cast<uint32_t*>(smem);
-    float* sO = reinterpret_cast<float*>(smem);                       // [warp][row][OROW]
+    float* sO = reinterpret_cast<float*>(smem);                                // [warp][row][OROW]
     float2* sML = reinterpret_cast<float2*>(sO + kWarps * S::ROWS * S::OROW);  // [warp][row]
     float* sScale = reinterpret_cast<float*>(smem + S::SMEM) - S::ROWS;
     __shared__ int s_next;
@@ -171,11 +188,110 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
         const int first_pos = p.context_lens[item.seq] - qlen;
         const int nrows = min(S::ROWS, qlen * p.group - item.row0);
         const int32_t* table = p.block_tables + int64_t(item.seq) * p.max_blocks;
+        const int pos_lo = first_pos + item.row0 / p.group;
+        const int pos_hi = first_pos + (item.row0 + nrows - 1) / p.group;
+
+        // ---- where the positions of a chunk live --------------------------------
+        // Only positions that some row of the tile sees are looked up: blocks that
+        // a window has left behind may be anyone's.
+        auto seen = [&](int j) {
+            return j <= pos_hi && (p.window <= 0 || j > pos_lo - p.window || j < p.sinks);
+        };
+        auto block_at = [&](int j) -> int {
+            const int b = table[j / p.a.block_size];
+            if (b >= 0 && b < p.a.num_blocks) return b;
+            raise_status(kStatusBounds);
+            return -1;
+        };
+        struct Where {
+            int blk;   // kB16: of the chunk; else of position lane % 16. < 0: none
+            int in;    // kB16: slot of the chunk's first position; else of lane % 16
+            int exps;  // a_j of position lane (< 16), b_j of position lane - 16
+            int base;  // first position
+        };
+        int ahead_blk = -1, ahead_in = 0;  // kB16: of the warp's next 32 chunks, one per lane
+        auto locate = [&](int c, int n) -> Where {  // entry c of the list, the warp's n-th
+            Where x;
+            x.base = kv8_chunk(item, c) * kChunk;
+            if constexpr (kB16) {
+                // block_size is a multiple of 16: a chunk lies in one block, and some
+                // row sees part of it
+                if ((n & 31) == 0) {
+                    const int cc = c + lane * kWarps;
+                    if (cc < item.c1) {
+                        const int j = kv8_chunk(item, cc) * kChunk;
+                        ahead_blk = block_at(j);
+                        ahead_in = j % p.a.block_size;
+                    }
+                }
+                x.blk = __shfl_sync(0xffffffffu, ahead_blk, n & 31);
+                x.in = __shfl_sync(0xffffffffu, ahead_in, n & 31);
+            } else {
+                const int j = x.base + (lane & 15);
+                x.blk = seen(j) ? block_at(j) : -1;
+                x.in = j % p.a.block_size;
+            }
+            x.exps = 0;
+            if (x.blk >= 0) {
+                const int8_t* e = lane < 16 ? p.a.k_exps : p.a.v_exps;
+                x.exps = __ldg(e + int64_t(x.blk) * p.a.exp_block_stride + int64_t(h) * p.a.block_size +
+                               (kB16 ? x.in + (lane & 15) : x.in));
+            }
+            return x;
+        };
+        const int64_t head = int64_t(h) * HD;
+        // byte offset of position `key` of the chunk (less the head's), < 0: none
+        auto row_of = [&](const Where& x, int key) -> int64_t {
+            if constexpr (kB16) {
+                return x.blk < 0 ? -1 : int64_t(x.blk) * p.a.block_stride + int64_t(x.in + key) * p.a.row;
+            } else {
+                const int blk = __shfl_sync(0xffffffffu, x.blk, key);
+                const int in = __shfl_sync(0xffffffffu, x.in, key);
+                return blk < 0 ? -1 : int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row;
+            }
+        };
+        Piece<F::KB> kr[ST][2][F::KP];
+        Piece<F::VB> vr[ST][4][F::VP];
+        auto load_k = [&](const Where& x, auto& dst) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t at = row_of(x, g + 8 * i);
+#pragma unroll
+                for (int q = 0; q < F::KP; ++q) {
+#pragma unroll
+                    for (int s = 0; s < F::KW; ++s) dst[i][q].w[s] = 0;
+                    if (at >= 0) dst[i][q] = load_piece<F::KB>(p.a.k_codes + head + at + (t + 4 * q) * F::KB);
+                }
+            }
+        };
+        auto load_v = [&](const Where& x, auto& dst) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = row_of(x, 2 * t + (i & 1) + 8 * (i >> 1));
+#pragma unroll
+                for (int q = 0; q < F::VP; ++q) {
+#pragma unroll
+                    for (int s = 0; s < F::VW; ++s) dst[i][q].w[s] = 0;
+                    if (at >= 0) dst[i][q] = load_piece<F::VB>(p.a.v_codes + head + at + (g + 8 * q) * F::VB);
+                }
+            }
+        };
+
+        Where wh[ST];
+#pragma unroll
+        for (int b = 0; b < ST; ++b) {
+            const int c = item.c0 + warp + b * kWarps;
+            wh[b].blk = -1;
+            if (c < item.c1) {
+                wh[b] = locate(c, b);
+                load_k(wh[b], kr[b]);
+                load_v(wh[b], vr[b]);
+            }
+        }
 
         // ---- Q: each row scaled to [1, 2), its terms stored as MMA fragments ----
-        // A warp takes a row at a time; element d of a lane's row goes where lane
-        // (g, t) of step (i, s) finds it: d = KB (t + 4 i) + 4 s + e, words e / 2 of
-        // the two row halves.
+        // Dim d of column n is what lane (n, t) of step (i, s) holds, d = KB (t + 4 i)
+        // + 4 s + e, as half e of its two words.
         for (int r = warp; r < S::ROWS; r += kWarps) {
             constexpr int PER = HD / 32;
             float x[PER];
@@ -194,311 +310,224 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             const int e = min(max(int(__float_as_uint(a) >> 23) - 127, -126), 126);
             const float inv = exp2_int(-e);
             if (lane == 0) sScale[r] = exp2_int(e) * p.qk_scale_log2;
-            const int mt = r / (16 / NT), rr = r % (16 / NT);
+            const int nq = r / (8 / NT), col = r % (8 / NT) * NT;
 #pragma unroll
             for (int d = 0; d < PER; ++d) {
                 const float v = x[d] * inv;
                 const int dim = d * 32 + lane;
                 const int piece = dim / F::KB, step = (piece >> 2) * F::KW + (dim % F::KB) / 4;
-                const int e4 = dim & 3;
-                // word (row half) + 2 (e4 / 2) of lane (rr % 8) * 4 + piece % 4
                 __half* dst = reinterpret_cast<__half*>(
-                    sQ + ((mt * F::KSTEPS + step) * 32 + (rr & 7) * 4 + (piece & 3)) * 4);
+                                  sQ + ((nq * F::KSTEPS + step) * 32 + col * 4 + (piece & 3)) * 2) + (dim & 3);
                 const __half hi = __float2half_rn(v);
-                dst[(e4 >> 1) * 4 + (NT == 2 ? 0 : rr >> 3) * 2 + (e4 & 1)] = hi;
-                if constexpr (NT == 2) {
-                    dst[(e4 >> 1) * 4 + 2 + (e4 & 1)] = __float2half_rn(v - __half2float(hi));
-                }
+                dst[0] = hi;
+                if constexpr (NT == 2) dst[16] = __float2half_rn(v - __half2float(hi));  // the next column
             }
         }
         __syncthreads();
-
-        // rows of this lane: scale, position (rows past the tile see nothing, and
-        // their zero Q keeps them finite)
-        float qs[MT][RL];
-        int pos[MT][RL];
+        uint2 qf[S::Q_REGS ? NQ : 1][S::Q_REGS ? F::KSTEPS : 1];
+        if constexpr (S::Q_REGS) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-            for (int i = 0; i < RL; ++i) {
-                const int r = mt * 8 * RL + i * 8 + g;
-                qs[mt][i] = sScale[r];
-                pos[mt][i] = first_pos + (item.row0 + min(r, nrows - 1)) / p.group;
-            }
-        const int pos_lo = first_pos + item.row0 / p.group;
-        const int pos_hi = first_pos + (item.row0 + nrows - 1) / p.group;
-
-        float m[MT][RL], l[MT][RL];
-        float o[MT][F::NTILES][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int i = 0; i < RL; ++i) {
-                m[mt][i] = -INFINITY;
-                l[mt][i] = 0.f;
-            }
-#pragma unroll
-            for (int n = 0; n < F::NTILES; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[mt][n][c] = 0.f;
+                for (int k = 0; k < F::KSTEPS; ++k) {
+                    qf[nq][k] = *reinterpret_cast<const uint2*>(sQ + ((nq * F::KSTEPS + k) * 32 + lane) * 2);
+                }
         }
 
-        // ---- where the positions of a chunk live --------------------------------
-        // Lane l holds, for position l % 16 of its chunk, block and slot (block < 0:
-        // a position past the tile's last one, or a block outside the arena).
-        int blk_ahead = 0;  // kB16: block of the warp's 32 next chunks, one per lane
-        auto block_at = [&](int j) -> int {  // block of position j
-            if (j > pos_hi) return -1;
-            const int b = table[j / p.a.block_size];
-            if (b < 0 || b >= p.a.num_blocks) {
-                raise_status(kStatusBounds);
-                return -1;
+        // rows of this lane: scale, position (rows past the tile see what its last
+        // one sees, and their zero Q keeps them finite)
+        float qs[NQ][RL], m[NQ][RL], l[NQ][RL];
+        int pos[NQ][RL];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int i = 0; i < RL; ++i) {
+                const int r = nq * (8 / NT) + t * RL + i;
+                qs[nq][i] = sScale[r];
+                pos[nq][i] = first_pos + (item.row0 + min(r, nrows - 1)) / p.group;
+                m[nq][i] = -INFINITY;
+                l[nq][i] = 0.f;
             }
-            return b;
-        };
-        struct Where {
-            int blk, in;  // of position lane % 16
-            int exps;     // kB16 or not: a_j of position lane (< 16), b_j of lane - 16
-            int base;     // first position
-        };
-        auto locate = [&](int c, int n) -> Where {  // entry c of the list, the warp's n-th
-            Where x;
-            x.base = kv8_chunk(item, c) * kChunk;
-            const int j = x.base + (lane & 15);
-            if constexpr (kB16) {
-                if ((n & 31) == 0) {
-                    const int cc = c + lane * kWarps;
-                    blk_ahead = cc < item.c1 ? block_at(kv8_chunk(item, cc) * kChunk) : -1;
-                }
-                x.blk = __shfl_sync(0xffffffffu, blk_ahead, n & 31);
-                x.in = j % p.a.block_size;
-                if (j > pos_hi) x.blk = -1;
-            } else {
-                x.blk = block_at(j);
-                x.in = j % p.a.block_size;
-            }
-            const int8_t* e = lane < 16 ? p.a.k_exps : p.a.v_exps;
-            x.exps = 0;
-            if (x.blk >= 0) x.exps = e[int64_t(x.blk) * p.a.exp_block_stride + int64_t(h) * p.a.block_size + x.in];
-            return x;
-        };
-        auto row_of = [&](const Where& x, int key, int& blk) -> int64_t {  // byte offset of the row
-            blk = __shfl_sync(0xffffffffu, x.blk, key);
-            const int in = __shfl_sync(0xffffffffu, x.in, key);
-            return int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + int64_t(h) * HD;
-        };
-        Piece<F::KB> kr[2][F::KP];
-        Piece<F::VB> vr[4][F::VP];
-        auto load_k = [&](const Where& x) {
+        float o[NQ][F::MTILES][OL];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                int blk;
-                const int64_t at = row_of(x, g + 8 * i, blk);
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int q = 0; q < F::KP; ++q) {
-                    if (blk >= 0) {
-                        kr[i][q] = load_piece<F::KB>(p.a.k_codes + at + (t + 4 * q) * F::KB);
-                    } else {
+            for (int k = 0; k < F::MTILES; ++k)
 #pragma unroll
-                        for (int s = 0; s < F::KW; ++s) kr[i][q].w[s] = 0;
-                    }
-                }
-            }
-        };
-        auto load_v = [&](const Where& x) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                int blk;
-                const int64_t at = row_of(x, 2 * t + (i & 1) + 8 * (i >> 1), blk);
-#pragma unroll
-                for (int q = 0; q < F::VP; ++q) {
-                    if (blk >= 0) {
-                        vr[i][q] = load_piece<F::VB>(p.a.v_codes + at + (g + 8 * q) * F::VB);
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < F::VW; ++s) vr[i][q].w[s] = 0;
-                    }
-                }
-            }
-        };
+                for (int e = 0; e < OL; ++e) o[nq][k][e] = 0.f;
 
-        int c = item.c0 + warp, n = 0;
-        Where cur{};
-        if (c < item.c1) {
-            cur = locate(c, n);
-            load_k(cur);
-            load_v(cur);
-        }
-        for (; c < item.c1; c += kWarps, ++n) {
-            // ---- S = Q K^T ------------------------------------------------------
-            float s[MT][2][4];
+        for (int c = item.c0 + warp, n = 0; c < item.c1;) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int b = 0; b < ST; ++b, c += kWarps, ++n) {
+                if (c >= item.c1) break;
+                // ---- S^T = K Q^T ------------------------------------------------
+                float s[NQ][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[mt][i][k] = 0.f;
+                    for (int k = 0; k < 4; ++k) s[nq][k] = 0.f;
 #pragma unroll
-            for (int q = 0; q < F::KP; ++q)
+                for (int q = 0; q < F::KP; ++q)
 #pragma unroll
-                for (int st = 0; st < F::KW; ++st) {
-                    uint32_t b[2][2];
-                    to_half4<kFormat>(kr[0][q].w[st], b[0][0], b[0][1]);
-                    to_half4<kFormat>(kr[1][q].w[st], b[1][0], b[1][1]);
+                    for (int st = 0; st < F::KW; ++st) {
+                        uint32_t a[4];
+                        to_half4<kFormat>(kr[b][0][q].w[st], a[0], a[2]);
+                        to_half4<kFormat>(kr[b][1][q].w[st], a[1], a[3]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const uint4 a = *reinterpret_cast<const uint4*>(
-                            sQ + ((mt * F::KSTEPS + q * F::KW + st) * 32 + lane) * 4);
-                        // words: (row g, dims 0 1), (row g + 8, 0 1), (g, 2 3), (g + 8, 2 3)
-                        const uint32_t f[4] = {a.x, a.y, a.z, a.w};
-                        mma(s[mt][0], f, b[0][0], b[0][1]);
-                        mma(s[mt][1], f, b[1][0], b[1][1]);
+                        for (int nq = 0; nq < NQ; ++nq) {
+                            const int step = q * F::KW + st;
+                            const uint2 f = S::Q_REGS ? qf[S::Q_REGS ? nq : 0][S::Q_REGS ? step : 0]
+                                                      : *reinterpret_cast<const uint2*>(
+                                                            sQ + ((nq * F::KSTEPS + step) * 32 + lane) * 2);
+                            mma(s[nq], a, f.x, f.y);
+                        }
                     }
+                const Where now = wh[b];
+                const bool more = c + ST * kWarps < item.c1;
+                if (more) {
+                    wh[b] = locate(c + ST * kWarps, n + ST);
+                    load_k(wh[b], kr[b]);
                 }
-            // the next chunk's K flies from here on
-            const Where now = cur;
-            const bool more = c + kWarps < item.c1;
-            if (more) {
-                cur = locate(c + kWarps, n + 1);
-                load_k(cur);
-            }
 
-            // ---- softmax ----------------------------------------------------------
-            // this lane's positions: base + 8 i + 2 t + e
-            float ka[2][2], vb[2][2];
+                // ---- softmax ------------------------------------------------------
+                // this lane's positions: base + g + 8 k
+                float ka[2], vb[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = 8 * i + 2 * t + e;
-                    ka[i][e] = exp2_int(min(max(__shfl_sync(0xffffffffu, now.exps, key), -126), 127));
-                    vb[i][e] = float(__shfl_sync(0xffffffffu, now.exps, key + 16));
+                for (int k = 0; k < 2; ++k) {
+                    ka[k] = exp2_int(min(max(__shfl_sync(0xffffffffu, now.exps, g + 8 * k), -126), 127));
+                    vb[k] = float(__shfl_sync(0xffffffffu, now.exps, g + 8 * k + 16));
                 }
-            const bool ragged = now.base + kChunk - 1 > pos_lo ||
-                                (p.window > 0 && now.base + p.window <= pos_hi && now.base + kChunk > p.sinks);
-            uint32_t pa[MT][4];
-            float alpha[MT][RL];
+                const bool ragged = now.base + kChunk - 1 > pos_lo ||
+                                    (p.window > 0 && now.base + p.window <= pos_hi && now.base + kChunk > p.sinks);
+                uint32_t pb[NQ][2];
+                float alpha[NQ][RL];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+                for (int nq = 0; nq < NQ; ++nq) {
+                    float pw[2][2];  // [position][column]
 #pragma unroll
-                for (int i = 0; i < RL; ++i) {
-                    float x[2][2];
-                    float top = -INFINITY;
+                    for (int i = 0; i < RL; ++i) {
+                        float x[2], top = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float d = NT == 2 ? s[mt][k][e] + s[mt][k][e + 2] : s[mt][k][2 * i + e];
-                            x[k][e] = (d * ka[k][e]) * qs[mt][i];
+                        for (int k = 0; k < 2; ++k) {
+                            const float d = NT == 2 ? s[nq][2 * k] + s[nq][2 * k + 1] : s[nq][2 * k + i];
+                            x[k] = (d * ka[k]) * qs[nq][i];
                             if (ragged) {
-                                const int j = now.base + 8 * k + 2 * t + e;
-                                const bool see = j <= pos[mt][i] &&
-                                                 (p.window <= 0 || j > pos[mt][i] - p.window || j < p.sinks);
-                                if (!see) x[k][e] = -INFINITY;
+                                const int j = now.base + g + 8 * k;
+                                const bool see = j <= pos[nq][i] &&
+                                                 (p.window <= 0 || j > pos[nq][i] - p.window || j < p.sinks);
+                                if (!see) x[k] = -INFINITY;
                             }
-                            top = fmaxf(top, x[k][e] + vb[k][e]);
+                            top = fmaxf(top, x[k] + vb[k]);
                         }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float mn = top > m[mt][i] + kMargin ? top : m[mt][i];
-                    const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-                    alpha[mt][i] = ex2(m[mt][i] - mu);
-                    m[mt][i] = mn;
-                    float sum = 0.f;
-                    float w2[2][2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                        for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+                        const float mn = top > m[nq][i] + kMargin ? top : m[nq][i];
+                        const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+                        alpha[nq][i] = ex2(m[nq][i] - mu);
+                        m[nq][i] = mn;
+                        float sum = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float y = x[k][e] - mu;
+                        for (int k = 0; k < 2; ++k) {
+                            const float y = x[k] - mu;
                             sum += ex2(y);
-                            w2[k][e] = ex2(y + vb[k][e]);
+                            pw[k][i] = ex2(y + vb[k]);
                         }
-                    l[mt][i] = fmaf(l[mt][i], alpha[mt][i], sum);
-                    if constexpr (NT == 2) {
-                        pa[mt][0] = pack_half(w2[0][0], w2[0][1]);
-                        pa[mt][2] = pack_half(w2[1][0], w2[1][1]);
-                        pa[mt][1] = pack_rest(w2[0][0], w2[0][1], pa[mt][0]);
-                        pa[mt][3] = pack_rest(w2[1][0], w2[1][1], pa[mt][2]);
-                    } else {
-                        pa[mt][i] = pack_half(w2[0][0], w2[0][1]);
-                        pa[mt][2 + i] = pack_half(w2[1][0], w2[1][1]);
+                        l[nq][i] = fmaf(l[nq][i], alpha[nq][i], sum);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if constexpr (NT == 2) {
+                            const float hi = __half2float(__float2half_rn(pw[k][0]));
+                            pw[k][1] = pw[k][0] - hi;
+                            pw[k][0] = hi;
+                        }
+                        pb[nq][k] = transpose8(pack_half(pw[k][0], pw[k][1]));
                     }
                 }
-            }
 
-            // ---- O += P V -----------------------------------------------------------
-            // fp32 rows: the products of a chunk are added in fp32 registers, since
-            // the tensor core's own accumulation truncates and a long context would
-            // add that up. Others accumulate in place.
-            if constexpr (NT == 1) {
-                bool grew = false;
+                // ---- O^T += V^T P^T -------------------------------------------------
+                if (kB16 && ragged) {
+                    // rows that nothing sees hold anything: a weight of 0 must meet a 0
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) grew |= alpha[mt][0] != 1.f || alpha[mt][1] != 1.f;
-                if (__any_sync(0xffffffffu, grew)) {
+                    for (int i = 0; i < 4; ++i) {
+                        if (!seen(now.base + 2 * t + (i & 1) + 8 * (i >> 1))) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                            for (int q = 0; q < F::VP; ++q)
 #pragma unroll
-                        for (int q = 0; q < F::NTILES; ++q)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[mt][q][e] *= alpha[mt][e >> 1];
+                                for (int st = 0; st < F::VW; ++st) vr[b][i][q].w[st] = 0;
+                        }
+                    }
                 }
-            }
+                // fp32 rows: the products of a chunk are added in fp32 registers,
+                // since the tensor core's own accumulation truncates and a long
+                // context would add that up. Others accumulate in place.
+                if constexpr (NT == 1) {
+                    bool grew = false;
 #pragma unroll
-            for (int q = 0; q < F::VP; ++q)
+                    for (int nq = 0; nq < NQ; ++nq) grew |= alpha[nq][0] != 1.f || alpha[nq][1] != 1.f;
+                    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                for (int st = 0; st < F::VW; ++st) {
-                    uint32_t b0[4], b1[4];  // of the 4 tiles of this word
-                    const uint32_t x0 = vr[0][q].w[st], x1 = vr[1][q].w[st];
-                    const uint32_t y0 = vr[2][q].w[st], y1 = vr[3][q].w[st];
-                    to_half4<kFormat>(__byte_perm(x0, x1, 0x5140), b0[0], b0[1]);
-                    to_half4<kFormat>(__byte_perm(x0, x1, 0x7362), b0[2], b0[3]);
-                    to_half4<kFormat>(__byte_perm(y0, y1, 0x5140), b1[0], b1[1]);
-                    to_half4<kFormat>(__byte_perm(y0, y1, 0x7362), b1[2], b1[3]);
+                        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int tile = (q * F::VW + st) * 4 + j;
+                            for (int k = 0; k < F::MTILES; ++k)
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            if constexpr (NT == 2) {
-                                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma(d, pa[mt], b0[j], b1[j]);
-                                o[mt][tile][0] = fmaf(o[mt][tile][0], alpha[mt][0], d[0] + d[2]);
-                                o[mt][tile][1] = fmaf(o[mt][tile][1], alpha[mt][0], d[1] + d[3]);
-                            } else {
-                                mma(o[mt][tile], pa[mt], b0[j], b1[j]);
+                                for (int e = 0; e < 4; ++e) o[nq][k][e] *= alpha[nq][e & 1];
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < F::VP; ++q)
+#pragma unroll
+                    for (int st = 0; st < F::VW; ++st) {
+                        uint32_t a[2][4];  // of the 2 tiles of this word
+                        const uint32_t x0 = vr[b][0][q].w[st], x1 = vr[b][1][q].w[st];
+                        const uint32_t y0 = vr[b][2][q].w[st], y1 = vr[b][3][q].w[st];
+                        to_half4<kFormat>(__byte_perm(x0, x1, 0x5140), a[0][0], a[0][1]);
+                        to_half4<kFormat>(__byte_perm(x0, x1, 0x7362), a[1][0], a[1][1]);
+                        to_half4<kFormat>(__byte_perm(y0, y1, 0x5140), a[0][2], a[0][3]);
+                        to_half4<kFormat>(__byte_perm(y0, y1, 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int tile = (q * F::VW + st) * 2 + j;
+#pragma unroll
+                            for (int nq = 0; nq < NQ; ++nq) {
+                                if constexpr (NT == 2) {
+                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma(d, a[j], pb[nq][0], pb[nq][1]);
+                                    o[nq][tile][0] = fmaf(o[nq][tile][0], alpha[nq][0], d[0] + d[1]);
+                                    o[nq][tile][1] = fmaf(o[nq][tile][1], alpha[nq][0], d[2] + d[3]);
+                                } else {
+                                    mma(o[nq][tile], a[j], pb[nq][0], pb[nq][1]);
+                                }
                             }
                         }
                     }
-                }
-            if (more) load_v(cur);
+                if (more) load_v(wh[b], vr[b]);
+            }
         }
 
         // ---- join the warps ---------------------------------------------------------
         __syncthreads();  // Q's fragments are read no more
-        // Lane (g, t) holds, of tile (q, j), dims VB (2t + e) + 8 VB q + j of rows g (+ 8)
+        // Lane (g, t) holds dims VB g + 8 VB q + 2 k + e (tile (q, k), half e) of its rows
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
             for (int i = 0; i < RL; ++i) {
-                float sum = l[mt][i];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const int r = mt * 8 * RL + i * 8 + g;
-                if (t == 0) sML[warp * S::ROWS + r] = make_float2(m[mt][i], sum);
+                float sum = l[nq][i];
+#pragma unroll
+                for (int q = 4; q < 32; q <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
+                const int r = nq * (8 / NT) + t * RL + i;
+                if (g == 0) sML[warp * S::ROWS + r] = make_float2(m[nq][i], sum);
                 float* dst = sO + (warp * S::ROWS + r) * S::OROW;
 #pragma unroll
                 for (int q = 0; q < F::VP; ++q)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int j = 0; j < F::VB; j += 4) {
-                            const int tile = q * F::VB + j;
-                            const int k = NT == 2 ? e : 2 * i + e;
-                            *reinterpret_cast<float4*>(dst + F::VB * (2 * t + e) + 8 * F::VB * q + j) =
-                                make_float4(o[mt][tile][k], o[mt][tile + 1][k], o[mt][tile + 2][k],
-                                            o[mt][tile + 3][k]);
-                        }
+                    for (int j = 0; j < F::VB; j += 4) {
+                        const int k = (q * F::VB + j) / 2;
+                        *reinterpret_cast<float4*>(dst + F::VB * g + 8 * F::VB * q + j) =
+                            NT == 2 ? make_float4(o[nq][k][0], o[nq][k][1], o[nq][k + 1][0], o[nq][k + 1][1])
+                                    : make_float4(o[nq][k][i], o[nq][k][OL / 2 + i], o[nq][k + 1][i],
+                                                  o[nq][k + 1][OL / 2 + i]);
+                    }
             }
         __syncthreads();
         for (int r = warp; r < nrows; r += kWarps) {
@@ -538,10 +567,10 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     }
 }
 
-template <typename T, int kFormat, int HD, int MT, bool kB16>
+template <typename T, int kFormat, int HD, int NQ, bool kB16>
 cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
-    auto* k = kv8_attention_kernel<T, kFormat, HD, MT, kB16>;
-    constexpr size_t smem = Tile<T, HD, MT>::SMEM;
+    auto* k = kv8_attention_kernel<T, kFormat, HD, NQ, kB16>;
+    constexpr size_t smem = Tile<T, HD, NQ>::SMEM;
     static int grid_per_device[64] = {0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -560,17 +589,22 @@ cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t
     return launch_programmatic(k, dim3(unsigned(grid_per_device[dev])), dim3(kWarps * 32), smem, st, p, w);
 }
 
+template <typename T, int kFormat, int HD, int NQ>
+cudaError_t launch_blocks(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
+    return p.a.block_size % kChunk == 0 ? launch_kernel<T, kFormat, HD, NQ, true>(p, w, st)
+                                        : launch_kernel<T, kFormat, HD, NQ, false>(p, w, st);
+}
+
 template <typename T, int kFormat, int HD>
 cudaError_t launch_tile(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
-    const bool b16 = p.a.block_size % kChunk == 0;
-    if constexpr (HD <= 128) {
-        if (w.tile_rows > 16 / terms<T>()) {
-            return b16 ? launch_kernel<T, kFormat, HD, 2, true>(p, w, st)
-                       : launch_kernel<T, kFormat, HD, 2, false>(p, w, st);
-        }
+    switch (w.tile_rows * terms<T>() / 8) {
+        case 1: return launch_blocks<T, kFormat, HD, 1>(p, w, st);
+        case 2: return launch_blocks<T, kFormat, HD, 2>(p, w, st);
+        case 4:
+            if constexpr (HD <= 128) return launch_blocks<T, kFormat, HD, 4>(p, w, st);
+            break;
     }
-    return b16 ? launch_kernel<T, kFormat, HD, 1, true>(p, w, st)
-               : launch_kernel<T, kFormat, HD, 1, false>(p, w, st);
+    return cudaErrorInvalidValue;
 }
 
 template <typename T, int kFormat>
@@ -593,9 +627,9 @@ cudaError_t launch_type(const Kv8AttnParams& p, const Kv8Work& w, int32_t format
 // The work list's shape for these rows.
 Kv8Work work_for(int32_t max_query_len, int32_t group, int32_t dtype, int32_t head_dim) {
     Kv8Work w{};
-    const int one = dtype == NVLLM_DTYPE_FP32 ? 8 : 16;  // rows of one 16-row MMA tile
-    const bool two = head_dim <= 128 && int64_t(max_query_len) * group > one;
-    w.tile_rows = two ? 2 * one : one;
+    const int one = dtype == NVLLM_DTYPE_FP32 ? 4 : 8;  // rows of 8 MMA columns
+    const int64_t rows = int64_t(max_query_len) * group;
+    w.tile_rows = rows <= one ? one : rows <= 2 * one || head_dim > 128 ? 2 * one : 4 * one;
     w.chunk = kChunk;
     w.min_run = 32;
     w.target = 148 * 3 * 5;

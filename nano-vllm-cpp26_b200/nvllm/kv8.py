@@ -23,6 +23,7 @@ KV8_INT8 = 1
 
 _DTYPES = {}  # torch dtype -> nvllm_dtype, filled at the first call
 _FORMATS = {}  # torch dtype of the codes -> nvllm_kv8_format
+_INT32 = _RAW_STREAM = _CURRENT_DEVICE = None  # of torch, likewise
 
 
 class _Arena(ctypes.Structure):
@@ -37,7 +38,7 @@ _BOUND = None
 
 
 def _lib():
-    global _BOUND
+    global _BOUND, _INT32, _RAW_STREAM, _CURRENT_DEVICE
     if _BOUND is not None:
         return _BOUND
     import torch
@@ -53,6 +54,9 @@ def _lib():
     L.nvllm_kv8_attention.restype = ctypes.c_int
     L.nvllm_kv8_attention.argtypes = [vp, i64, vp, i64, i32, ap, vp, i32, vp, vp, i32, i32, i32, i32,
                                       i32, f32, i32, i32, vp, sz, lp, vp]
+    _INT32, _CURRENT_DEVICE = torch.int32, torch.cuda.current_device
+    _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda index: torch.cuda.current_stream(index).cuda_stream)
     _DTYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
     _FORMATS.update({torch.float8_e4m3fn: KV8_E4M3, torch.int8: KV8_INT8})
     _BOUND = L
@@ -85,7 +89,7 @@ class KV8Arena:
         if not k.is_cuda or any(t.device != k.device for t in (v, k_exp, v_exp)):
             raise ValueError("the arenas must be CUDA tensors on one device")
         self.layout, self.k, self.v, self.k_exp, self.v_exp = layout, k, v, k_exp, v_exp
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self._c = _Arena(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(),
                          _FORMATS[k.dtype])
         self._ref, self._lay = ctypes.byref(self._c), ctypes.byref(layout)
@@ -106,7 +110,7 @@ class KV8Arena:
 
 def _rows(t, name: str, width: int, arena: KV8Arena) -> int:
     """Checks a 2-d row tensor; its nvllm_dtype."""
-    if t.device != arena.device:
+    if t.get_device() != arena.index:
         raise ValueError(f"{name} must be on the arena's device {arena.device}, got {t.device}")
     kind = _DTYPES.get(t.dtype)
     if kind is None:
@@ -119,9 +123,9 @@ def _rows(t, name: str, width: int, arena: KV8Arena) -> int:
 
 
 def _ints(t, name: str, arena: KV8Arena, dim: int = 1):
-    if t.device != arena.device:
+    if t.get_device() != arena.index:
         raise ValueError(f"{name} must be on the arena's device {arena.device}, got {t.device}")
-    if str(t.dtype) != "torch.int32":
+    if t.dtype != _INT32:
         raise ValueError(f"{name} must be int32, got {t.dtype}")
     if t.dim() != dim or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dim}-d tensor")
@@ -134,12 +138,16 @@ def _stride(t) -> int:
 
 def _call(arena: KV8Arena, stream, f, *args) -> int:
     """Calls f(*args, stream) with the arena's device current."""
+    if stream is None:
+        # the raw handle: a Stream object costs more than the launch
+        stream = _RAW_STREAM(arena.index)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    if arena.index == _CURRENT_DEVICE():
+        return f(*args, stream)
     import torch
-    dev = arena.device.index
-    if dev is None or dev == torch.cuda.current_device():
-        return f(*args, _nv._stream_ptr(stream))
-    with torch.cuda.device(dev):
-        return f(*args, _nv._stream_ptr(stream))
+    with torch.cuda.device(arena.index):
+        return f(*args, stream)
 
 
 def _move(what: str, f, key, value, arena: KV8Arena, slot_mapping, layer: int, stream,
@@ -207,6 +215,8 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
     kind = _rows(query, "query", width, arena)
     if _rows(out, "out", width, arena) != kind:
         raise ValueError(f"out must have query's type {query.dtype}, got {out.dtype}")
+    if out.shape[0] < query.shape[0]:
+        raise ValueError(f"out must hold query's {query.shape[0]} rows")
     _ints(block_tables, "block_tables", arena, 2)
     _ints(cu_seqlens_q, "cu_seqlens_q", arena)
     _ints(context_lens, "context_lens", arena)
@@ -220,7 +230,7 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
                                         arena.device)
         if stream is not None and not isinstance(stream, int):
             workspace.record_stream(stream)  # it is freed here, in use there
-    elif workspace.device != arena.device:
+    elif workspace.get_device() != arena.index:
         raise ValueError(f"workspace must be on the arena's device {arena.device}")
     st = _call(arena, stream, _lib().nvllm_kv8_attention, out.data_ptr(), _stride(out),
                query.data_ptr(), _stride(query), kind, arena._ref, block_tables.data_ptr(),

@@ -273,6 +273,20 @@ def test_window_and_sinks(nv, torch, dtype, window, sinks, seqs, heads, kv, hd):
     b.check()
 
 
+@pytest.mark.parametrize("block", [1, 8, 16, 24, 32])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("seqs", [[(1, 700), (1, 90)], [(7, 400), (90, 600)]], ids=["decodes", "chunks"])
+def test_blocks_behind_the_window_are_not_read(nv, torch, block, dtype, seqs):
+    """Table entries of blocks that no row sees any part of may hold anything."""
+    b = Batch(nv, torch, seqs, 4, 2, 128, block=block, dtype=dtype, window=70, sinks=5, seed=block)
+    for s, (new, ctx) in enumerate(seqs):
+        first = ctx - new - 70 + 1  # of the first row's window
+        for i in range(-(-5 // block), max(0, first) // block):
+            b.tables[s, i] = -9 if i % 2 else 1 << 30
+    b.call()
+    b.check()
+
+
 @pytest.mark.parametrize("block", [1, 3, 8, 24, 32, 100])
 @pytest.mark.parametrize("seqs", [DECODES, CHUNKS], ids=["decodes", "chunks"])
 @pytest.mark.parametrize("hd", [64, 128])
