@@ -25,14 +25,15 @@
 // 8 x 8 transpose (movmatrix).
 //
 // What bounds a decode is the cache's bytes. A CTA of 4 warps takes runs of
-// chunks (kv8_plan.cu); a warp takes every fourth chunk of 16 positions and
-// loads its fragments straight from the arenas: of K, lane (g, t) the 16-byte
-// pieces t, t + 4, .. of rows g and g + 8 (the MMA's order of the dims is
-// permuted to match, Q's fragments are stored that way); of V, the pieces of
-// dims g of rows 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes are paired across rows
-// as they are converted. No shared memory and no bank conflicts on the way; a
-// stage's registers are loaded again as soon as they are converted, STAGES chunks
-// ahead. The warps' results are joined through shared memory at the end of a run.
+// chunks (kv8_plan.cu); a warp takes every fourth chunk of SUB x 16 positions and
+// brings them into its own two shared-memory buffers by 16-byte asynchronous
+// copies (positions that no row sees as zeros), one chunk in flight while it
+// computes the other. Of K, lane (g, t) reads the pieces t, t + 4, .. of rows g
+// and g + 8 (the MMA's order of the dims is permuted to match, Q's fragments are
+// stored that way); of V, the piece g of rows 2t, 2t + 1, 2t + 8, 2t + 9, whose
+// bytes are paired across rows as they are converted. Pieces are placed so that
+// both reads are free of bank conflicts (Ring::swizzle). The warps' results are
+// joined through shared memory at the end of a run.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -42,7 +43,7 @@ namespace nvllm {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kChunk = 16;
+constexpr int kSub = 16;  // positions of one MMA tile
 
 template <typename T>
 constexpr int terms() { return sizeof(T) == 4 ? 2 : 1; }
@@ -65,20 +66,29 @@ struct Piece {
     uint32_t w[BYTES / 4];
 };
 
-// Read once by this tile: do not keep it in L1.
 template <int BYTES>
-__device__ __forceinline__ Piece<BYTES> load_piece(const unsigned char* p) {
+__device__ __forceinline__ Piece<BYTES> read_piece(const unsigned char* p) {
     Piece<BYTES> r;
     if constexpr (BYTES == 16) {
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
-                     : "l"(p));
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
     } else if constexpr (BYTES == 8) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = v.x; r.w[1] = v.y;
     } else {
-        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
+        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
     return r;
+}
+
+// 16 bytes, or zeros where there is nothing to read.
+__device__ __forceinline__ void copy16(uint32_t dst, const unsigned char* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Four codes -> two pairs of fp16, in order.
@@ -136,18 +146,48 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // this (log2): until then P <= 2^margin, and it cancels in acc / l.
 constexpr float kMargin = 4.0f;
 
+// 16-position tiles per chunk: independent work between a warp's few, long
+// dependences (a maximum over lanes, a rescale), as far as registers go.
+constexpr int subs(int head_dim, int nq) {
+    return nq > 2 || head_dim == 256 ? 1 : head_dim == 128 || nq == 2 ? 2 : 4;
+}
+
+// One 16-position tile of K or V in shared memory: rows of HD bytes, the 16-byte
+// pieces of a 128-byte line permuted by its rows. K's reads take 8 / (HD / 16)
+// neighbouring rows' pieces at once, V's the same pieces of rows 0, 2, 4, 6: the
+// permutation gives both all eight places of a line.
+template <int HD>
+struct Ring {
+    static constexpr int TILE = kSub * HD;
+    static constexpr int PIECES = HD / 16;           // of a row
+    static constexpr int STEP = 32 / PIECES;         // rows that the lanes of a warp copy at once
+    static constexpr int COPIES = kSub / STEP;       // per lane and tile
+    __device__ static __forceinline__ int swizzle(int row) {
+        if constexpr (HD >= 128) return ((row >> 1) & 3) * 2 ^ (row & 1) * 4;
+        if constexpr (HD == 64) return ((row >> 1) & 3) * 2;
+        return ((row >> 2) & 1) * 2;
+    }
+    // byte offset of byte `b` of row `row`
+    __device__ static __forceinline__ int at(int row, int b) {
+        return (row * HD + b) ^ (swizzle(row) * 16);
+    }
+};
+
 template <typename T, int HD, int NQ>
 struct Tile {
     static constexpr int ROWS = NQ * 8 / terms<T>();   // rows of a query tile
     static constexpr int Q_WORDS = NQ * (HD / 16) * 64;  // fragments of Q
-    static constexpr bool Q_REGS = NQ * (HD / 16) <= 16; // held in registers
-    // chunks in flight per warp, as far as registers go
-    static constexpr int STAGES = HD == 256 || NQ > 2 || (HD == 128 && NQ > 1) ? 1 : 2;
+    static constexpr bool Q_REGS = NQ * (HD / 16) <= 8;  // held in registers
+    static constexpr int SUB = subs(HD, NQ);
     static constexpr int OROW = HD + 4;
-    // the warps' results overlay Q's fragments
-    static constexpr size_t JOIN = size_t(kWarps) * ROWS * (OROW + 2) * 4;
-    static constexpr size_t SMEM = (Q_WORDS * 4 > JOIN ? Q_WORDS * 4 : JOIN) + ROWS * 4;
-    static constexpr int CTAS = HD * NQ >= 256 ? 2 : HD * NQ > 64 ? 3 : 4;
+    static constexpr size_t BUF = 2 * SUB * Ring<HD>::TILE;        // K and V of a chunk
+    static constexpr size_t RING = kWarps * 2 * BUF;
+    static constexpr size_t JOIN = size_t(kWarps) * ROWS * (OROW + 2) * 4;  // overlays the buffers
+    static constexpr size_t EXPS = RING > JOIN ? RING : JOIN;      // factors of a chunk's positions
+    static constexpr size_t Q = EXPS + kWarps * 2 * SUB * 32 * 4;
+    static constexpr size_t SCALE = Q + Q_WORDS * 4;
+    static constexpr size_t SMEM = SCALE + ROWS * 4;
+    static constexpr int CTAS = HD * NQ >= 512 || HD == 256 ? 2 : 3;
 };
 
 template <typename T, int kFormat, int HD, int NQ, bool kB16>
@@ -158,18 +198,22 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     constexpr int NT = terms<T>();
     constexpr int RL = NT == 2 ? 1 : 2;    // rows of a lane per 8 columns
     constexpr int OL = NT == 2 ? 2 : 4;    // sums of a lane per 16 x 8 tile of O^T
-    constexpr int ST = S::STAGES;
+    constexpr int SUB = S::SUB;
+    constexpr int CHUNK = SUB * kSub;
     extern __shared__ __align__(16) unsigned char smem[];
-    uint32_t* sQ = reinterpret_cast<uint32_t*>(smem);
+    uint32_t* sQ = reinterpret_cast<uint32_t*>(smem + S::Q);
     float* sO = reinterpret_cast<float*>(smem);                                // [warp][row][OROW]
     float2* sML = reinterpret_cast<float2*>(sO + kWarps * S::ROWS * S::OROW);  // [warp][row]
-    float* sScale = reinterpret_cast<float*>(smem + S::SMEM) - S::ROWS;
+    float* sScale = reinterpret_cast<float*>(smem + S::SCALE);
     __shared__ int s_next;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2;
     const int t = lane & 3;
+    using R = Ring<HD>;
+    unsigned char* ring = smem + warp * 2 * S::BUF;  // [buffer][tile][K, V]
+    float* sE = reinterpret_cast<float*>(smem + S::EXPS) + warp * 2 * SUB * 32;  // [buffer][tile][lane]
     pdl_release();
     pdl_wait();  // the work list, the rows and the cache come from the kernels before
     const int H = p.a.num_heads;
@@ -204,30 +248,32 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             return -1;
         };
         struct Where {
-            int blk;   // kB16: of the chunk; else of position lane % 16. < 0: none
-            int in;    // kB16: slot of the chunk's first position; else of lane % 16
+            int blk;   // kB16: of the 16 positions; else of position lane % 16. < 0: none
+            int in;    // kB16: slot of the first; else of position lane % 16
             int exps;  // a_j of position lane (< 16), b_j of position lane - 16
-            int base;  // first position
         };
-        int ahead_blk = -1, ahead_in = 0;  // kB16: of the warp's next 32 chunks, one per lane
-        auto locate = [&](int c, int n) -> Where {  // entry c of the list, the warp's n-th
+        int ahead_blk = -1, ahead_in = 0;  // kB16: of the warp's next 32 tiles of 16, one per lane
+        auto base_of = [&](int c) { return kv8_chunk(item, c) * CHUNK; };
+        auto locate = [&](int c, int n, int u) -> Where {  // tile u of entry c, the warp's n-th
             Where x;
-            x.base = kv8_chunk(item, c) * kChunk;
             if constexpr (kB16) {
-                // block_size is a multiple of 16: a chunk lies in one block, and some
-                // row sees part of it
-                if ((n & 31) == 0) {
-                    const int cc = c + lane * kWarps;
+                // block_size is a multiple of 16: 16 positions lie in one block
+                const int at = n * SUB + u;
+                if ((at & 31) == 0) {
+                    const int cc = c + (lane / SUB) * kWarps;
+                    ahead_blk = -1;
                     if (cc < item.c1) {
-                        const int j = kv8_chunk(item, cc) * kChunk;
-                        ahead_blk = block_at(j);
-                        ahead_in = j % p.a.block_size;
+                        const int j = base_of(cc) + lane % SUB * kSub;
+                        if (j <= pos_hi && (p.window <= 0 || j + kSub - 1 > pos_lo - p.window || j < p.sinks)) {
+                            ahead_blk = block_at(j);
+                            ahead_in = j % p.a.block_size;
+                        }
                     }
                 }
-                x.blk = __shfl_sync(0xffffffffu, ahead_blk, n & 31);
-                x.in = __shfl_sync(0xffffffffu, ahead_in, n & 31);
+                x.blk = __shfl_sync(0xffffffffu, ahead_blk, at & 31);
+                x.in = __shfl_sync(0xffffffffu, ahead_in, at & 31);
             } else {
-                const int j = x.base + (lane & 15);
+                const int j = base_of(c) + u * kSub + (lane & 15);
                 x.blk = seen(j) ? block_at(j) : -1;
                 x.in = j % p.a.block_size;
             }
@@ -239,54 +285,53 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             }
             return x;
         };
-        const int64_t head = int64_t(h) * HD;
-        // byte offset of position `key` of the chunk (less the head's), < 0: none
-        auto row_of = [&](const Where& x, int key) -> int64_t {
-            if constexpr (kB16) {
-                return x.blk < 0 ? -1 : int64_t(x.blk) * p.a.block_stride + int64_t(x.in + key) * p.a.row;
-            } else {
-                const int blk = __shfl_sync(0xffffffffu, x.blk, key);
-                const int in = __shfl_sync(0xffffffffu, x.in, key);
-                return blk < 0 ? -1 : int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row;
-            }
+        // starts the copies of entry c into buffer b; its exponents come back
+        struct Exps {
+            int e[SUB];
         };
-        Piece<F::KB> kr[ST][2][F::KP];
-        Piece<F::VB> vr[ST][4][F::VP];
-        auto load_k = [&](const Where& x, auto& dst) {
+        const int64_t piece = int64_t(h) * HD + lane % R::PIECES * 16;
+        auto issue = [&](int c, int n, int b) -> Exps {
+            Exps r;
+            const int base = base_of(c);
+            const bool all = base >= 0 && base + CHUNK - 1 <= pos_hi &&
+                             (p.window <= 0 || base > pos_lo - p.window || base + CHUNK <= p.sinks);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t at = row_of(x, g + 8 * i);
+            for (int u = 0; u < SUB; ++u) {
+                const Where x = locate(c, n, u);
+                r.e[u] = x.exps;
+                const uint32_t dst = smem_addr(ring + b * S::BUF + u * 2 * R::TILE);
 #pragma unroll
-                for (int q = 0; q < F::KP; ++q) {
-#pragma unroll
-                    for (int s = 0; s < F::KW; ++s) dst[i][q].w[s] = 0;
-                    if (at >= 0) dst[i][q] = load_piece<F::KB>(p.a.k_codes + head + at + (t + 4 * q) * F::KB);
+                for (int i = 0; i < R::COPIES; ++i) {
+                    const int row = lane / R::PIECES + i * R::STEP;
+                    int blk = x.blk, in = x.in + row;
+                    if constexpr (!kB16) {
+                        blk = __shfl_sync(0xffffffffu, x.blk, row);
+                        in = __shfl_sync(0xffffffffu, x.in, row);
+                    }
+                    const bool on = blk >= 0 && (!kB16 || all || seen(base + u * kSub + row));
+                    const int64_t at = on ? int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + piece : 0;
+                    const uint32_t to = dst + R::at(row, lane % R::PIECES * 16);
+                    copy16(to, p.a.k_codes + at, on);
+                    copy16(to + R::TILE, p.a.v_codes + at, on);
                 }
             }
+            return r;
         };
-        auto load_v = [&](const Where& x, auto& dst) {
+        auto store_exps = [&](const Exps& x, int b) {  // 2^a_j of the 16 positions, then b_j
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t at = row_of(x, 2 * t + (i & 1) + 8 * (i >> 1));
-#pragma unroll
-                for (int q = 0; q < F::VP; ++q) {
-#pragma unroll
-                    for (int s = 0; s < F::VW; ++s) dst[i][q].w[s] = 0;
-                    if (at >= 0) dst[i][q] = load_piece<F::VB>(p.a.v_codes + head + at + (g + 8 * q) * F::VB);
-                }
+            for (int u = 0; u < SUB; ++u) {
+                sE[(b * SUB + u) * 32 + lane] = lane < 16 ? exp2_int(min(max(x.e[u], -126), 127)) : float(x.e[u]);
             }
         };
-
-        Where wh[ST];
-#pragma unroll
-        for (int b = 0; b < ST; ++b) {
-            const int c = item.c0 + warp + b * kWarps;
-            wh[b].blk = -1;
-            if (c < item.c1) {
-                wh[b] = locate(c, b);
-                load_k(wh[b], kr[b]);
-                load_v(wh[b], vr[b]);
-            }
+        Exps ahead{};
+        {
+            const int c = item.c0 + warp;
+            Exps first{};
+            if (c < item.c1) first = issue(c, 0, 0);
+            copy_commit();
+            if (c + kWarps < item.c1) ahead = issue(c + kWarps, 1, 1);
+            copy_commit();
+            store_exps(first, 0);
         }
 
         // ---- Q: each row scaled to [1, 2), its terms stored as MMA fragments ----
@@ -356,157 +401,189 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                 for (int e = 0; e < OL; ++e) o[nq][k][e] = 0.f;
 
-        for (int c = item.c0 + warp, n = 0; c < item.c1;) {
+        for (int c = item.c0 + warp, n = 0; c < item.c1; c += kWarps, ++n) {
+            const int buf = n & 1;
+            copy_wait<1>();
+            store_exps(ahead, buf ^ 1);
+            __syncwarp();
+            const unsigned char* sK = ring + buf * S::BUF;
+            const unsigned char* sV = sK + R::TILE;
+            // ---- S^T = K Q^T ----------------------------------------------------
+            float s[NQ][SUB][4];
 #pragma unroll
-            for (int b = 0; b < ST; ++b, c += kWarps, ++n) {
-                if (c >= item.c1) break;
-                // ---- S^T = K Q^T ------------------------------------------------
-                float s[NQ][4];
+            for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int nq = 0; nq < NQ; ++nq)
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[nq][k] = 0.f;
+                    for (int k = 0; k < 4; ++k) s[nq][u][k] = 0.f;
 #pragma unroll
-                for (int q = 0; q < F::KP; ++q)
+            for (int q = 0; q < F::KP; ++q) {
+                Piece<F::KB> kr[SUB][2];
 #pragma unroll
-                    for (int st = 0; st < F::KW; ++st) {
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        kr[u][i] = read_piece<F::KB>(sK + u * 2 * R::TILE + R::at(g + 8 * i, (t + 4 * q) * F::KB));
+                    }
+#pragma unroll
+                for (int st = 0; st < F::KW; ++st) {
+                    const int step = q * F::KW + st;
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) {
                         uint32_t a[4];
-                        to_half4<kFormat>(kr[b][0][q].w[st], a[0], a[2]);
-                        to_half4<kFormat>(kr[b][1][q].w[st], a[1], a[3]);
+                        to_half4<kFormat>(kr[u][0].w[st], a[0], a[2]);
+                        to_half4<kFormat>(kr[u][1].w[st], a[1], a[3]);
 #pragma unroll
                         for (int nq = 0; nq < NQ; ++nq) {
-                            const int step = q * F::KW + st;
                             const uint2 f = S::Q_REGS ? qf[S::Q_REGS ? nq : 0][S::Q_REGS ? step : 0]
                                                       : *reinterpret_cast<const uint2*>(
                                                             sQ + ((nq * F::KSTEPS + step) * 32 + lane) * 2);
-                            mma(s[nq], a, f.x, f.y);
+                            mma(s[nq][u], a, f.x, f.y);
                         }
                     }
-                const Where now = wh[b];
-                const bool more = c + ST * kWarps < item.c1;
-                if (more) {
-                    wh[b] = locate(c + ST * kWarps, n + ST);
-                    load_k(wh[b], kr[b]);
                 }
-
-                // ---- softmax ------------------------------------------------------
-                // this lane's positions: base + g + 8 k
-                float ka[2], vb[2];
+            }
+            // this lane's positions: base + 16 u + g + 8 k
+            float ka[SUB][2], vb[SUB][2];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    ka[k] = exp2_int(min(max(__shfl_sync(0xffffffffu, now.exps, g + 8 * k), -126), 127));
-                    vb[k] = float(__shfl_sync(0xffffffffu, now.exps, g + 8 * k + 16));
+                    ka[u][k] = sE[(buf * SUB + u) * 32 + g + 8 * k];
+                    vb[u][k] = sE[(buf * SUB + u) * 32 + g + 8 * k + 16];
                 }
-                const bool ragged = now.base + kChunk - 1 > pos_lo ||
-                                    (p.window > 0 && now.base + p.window <= pos_hi && now.base + kChunk > p.sinks);
-                uint32_t pb[NQ][2];
-                float alpha[NQ][RL];
+
+            // ---- softmax ----------------------------------------------------------
+            const int base = base_of(c);
+            const bool ragged = base + CHUNK - 1 > pos_lo ||
+                                (p.window > 0 && base + p.window <= pos_hi && base + CHUNK > p.sinks);
+            uint32_t pb[NQ][SUB][2];
+            float alpha[NQ][RL];
 #pragma unroll
-                for (int nq = 0; nq < NQ; ++nq) {
-                    float pw[2][2];  // [position][column]
+            for (int nq = 0; nq < NQ; ++nq) {
+                float pw[SUB][2][2];  // [tile][position][column]
 #pragma unroll
-                    for (int i = 0; i < RL; ++i) {
-                        float x[2], top = -INFINITY;
+                for (int i = 0; i < RL; ++i) {
+                    float x[SUB][2], top = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const float d = NT == 2 ? s[nq][2 * k] + s[nq][2 * k + 1] : s[nq][2 * k + i];
-                            x[k] = (d * ka[k]) * qs[nq][i];
+                            const float d = NT == 2 ? s[nq][u][2 * k] + s[nq][u][2 * k + 1] : s[nq][u][2 * k + i];
+                            x[u][k] = (d * ka[u][k]) * qs[nq][i];
                             if (ragged) {
-                                const int j = now.base + g + 8 * k;
+                                const int j = base + u * kSub + g + 8 * k;
                                 const bool see = j <= pos[nq][i] &&
                                                  (p.window <= 0 || j > pos[nq][i] - p.window || j < p.sinks);
-                                if (!see) x[k] = -INFINITY;
+                                if (!see) x[u][k] = -INFINITY;
                             }
-                            top = fmaxf(top, x[k] + vb[k]);
+                            top = fmaxf(top, x[u][k] + vb[u][k]);
                         }
 #pragma unroll
-                        for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
-                        const float mn = top > m[nq][i] + kMargin ? top : m[nq][i];
-                        const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-                        alpha[nq][i] = ex2(m[nq][i] - mu);
-                        m[nq][i] = mn;
-                        float sum = 0.f;
+                    for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+                    const float mn = top > m[nq][i] + kMargin ? top : m[nq][i];
+                    const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+                    alpha[nq][i] = ex2(m[nq][i] - mu);
+                    m[nq][i] = mn;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const float y = x[k] - mu;
+                            const float y = x[u][k] - mu;
                             sum += ex2(y);
-                            pw[k][i] = ex2(y + vb[k]);
+                            pw[u][k][i] = ex2(y + vb[u][k]);
                         }
-                        l[nq][i] = fmaf(l[nq][i], alpha[nq][i], sum);
-                    }
+                    l[nq][i] = fmaf(l[nq][i], alpha[nq][i], sum);
+                }
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         if constexpr (NT == 2) {
-                            const float hi = __half2float(__float2half_rn(pw[k][0]));
-                            pw[k][1] = pw[k][0] - hi;
-                            pw[k][0] = hi;
+                            const float hi = __half2float(__float2half_rn(pw[u][k][0]));
+                            pw[u][k][1] = pw[u][k][0] - hi;
+                            pw[u][k][0] = hi;
                         }
-                        pb[nq][k] = transpose8(pack_half(pw[k][0], pw[k][1]));
+                        pb[nq][u][k] = transpose8(pack_half(pw[u][k][0], pw[u][k][1]));
                     }
-                }
+            }
 
-                // ---- O^T += V^T P^T -------------------------------------------------
-                if (kB16 && ragged) {
-                    // rows that nothing sees hold anything: a weight of 0 must meet a 0
+            // ---- O^T += V^T P^T -----------------------------------------------------
+            // fp32 rows: the products of a chunk are added in fp32 registers, since
+            // the tensor core's own accumulation truncates and a long context would
+            // add that up. Others accumulate in place.
+            if constexpr (NT == 1) {
+                bool grew = false;
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) grew |= alpha[nq][0] != 1.f || alpha[nq][1] != 1.f;
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int k = 0; k < F::MTILES; ++k)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[nq][k][e] *= alpha[nq][e & 1];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < F::VP; ++q) {
+                Piece<F::VB> vr[SUB][4];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (!seen(now.base + 2 * t + (i & 1) + 8 * (i >> 1))) {
-#pragma unroll
-                            for (int q = 0; q < F::VP; ++q)
-#pragma unroll
-                                for (int st = 0; st < F::VW; ++st) vr[b][i][q].w[st] = 0;
-                        }
+                        vr[u][i] = read_piece<F::VB>(sV + u * 2 * R::TILE +
+                                                     R::at(2 * t + (i & 1) + 8 * (i >> 1), (g + 8 * q) * F::VB));
                     }
-                }
-                // fp32 rows: the products of a chunk are added in fp32 registers,
-                // since the tensor core's own accumulation truncates and a long
-                // context would add that up. Others accumulate in place.
-                if constexpr (NT == 1) {
-                    bool grew = false;
 #pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq) grew |= alpha[nq][0] != 1.f || alpha[nq][1] != 1.f;
-                    if (__any_sync(0xffffffffu, grew)) {
+                for (int st = 0; st < F::VW; ++st) {
+                    float d[NQ][2][4];  // fp32 rows: this chunk's products
+                    if constexpr (NT == 2) {
 #pragma unroll
                         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                            for (int k = 0; k < F::MTILES; ++k)
+                            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[nq][k][e] *= alpha[nq][e & 1];
+                                for (int e = 0; e < 4; ++e) d[nq][j][e] = 0.f;
                     }
-                }
 #pragma unroll
-                for (int q = 0; q < F::VP; ++q)
-#pragma unroll
-                    for (int st = 0; st < F::VW; ++st) {
+                    for (int u = 0; u < SUB; ++u) {
                         uint32_t a[2][4];  // of the 2 tiles of this word
-                        const uint32_t x0 = vr[b][0][q].w[st], x1 = vr[b][1][q].w[st];
-                        const uint32_t y0 = vr[b][2][q].w[st], y1 = vr[b][3][q].w[st];
+                        const uint32_t x0 = vr[u][0].w[st], x1 = vr[u][1].w[st];
+                        const uint32_t y0 = vr[u][2].w[st], y1 = vr[u][3].w[st];
                         to_half4<kFormat>(__byte_perm(x0, x1, 0x5140), a[0][0], a[0][1]);
                         to_half4<kFormat>(__byte_perm(x0, x1, 0x7362), a[1][0], a[1][1]);
                         to_half4<kFormat>(__byte_perm(y0, y1, 0x5140), a[0][2], a[0][3]);
                         to_half4<kFormat>(__byte_perm(y0, y1, 0x7362), a[1][2], a[1][3]);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int tile = (q * F::VW + st) * 2 + j;
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
                             for (int nq = 0; nq < NQ; ++nq) {
-                                if constexpr (NT == 2) {
-                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma(d, a[j], pb[nq][0], pb[nq][1]);
-                                    o[nq][tile][0] = fmaf(o[nq][tile][0], alpha[nq][0], d[0] + d[1]);
-                                    o[nq][tile][1] = fmaf(o[nq][tile][1], alpha[nq][0], d[2] + d[3]);
-                                } else {
-                                    mma(o[nq][tile], a[j], pb[nq][0], pb[nq][1]);
-                                }
+                                float* sum = NT == 2 ? d[nq][j] : o[nq][(q * F::VW + st) * 2 + j];
+                                mma(sum, a[j], pb[nq][u][0], pb[nq][u][1]);
                             }
-                        }
                     }
-                if (more) load_v(wh[b], vr[b]);
+                    if constexpr (NT == 2) {
+#pragma unroll
+                        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                float* sum = o[nq][(q * F::VW + st) * 2 + j];
+                                sum[0] = fmaf(sum[0], alpha[nq][0], d[nq][j][0] + d[nq][j][1]);
+                                sum[1] = fmaf(sum[1], alpha[nq][0], d[nq][j][2] + d[nq][j][3]);
+                            }
+                    }
+                }
             }
+            __syncwarp();  // the buffer is free
+            if (c + 2 * kWarps < item.c1) ahead = issue(c + 2 * kWarps, n + 2, buf);
+            copy_commit();
         }
 
         // ---- join the warps ---------------------------------------------------------
-        __syncthreads();  // Q's fragments are read no more
+        copy_wait<0>();
+        __syncthreads();  // the buffers are read no more
         // Lane (g, t) holds dims VB g + 8 VB q + 2 k + e (tile (q, k), half e) of its rows
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
@@ -591,7 +668,7 @@ cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t
 
 template <typename T, int kFormat, int HD, int NQ>
 cudaError_t launch_blocks(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
-    return p.a.block_size % kChunk == 0 ? launch_kernel<T, kFormat, HD, NQ, true>(p, w, st)
+    return p.a.block_size % kSub == 0 ? launch_kernel<T, kFormat, HD, NQ, true>(p, w, st)
                                         : launch_kernel<T, kFormat, HD, NQ, false>(p, w, st);
 }
 
@@ -630,8 +707,8 @@ Kv8Work work_for(int32_t max_query_len, int32_t group, int32_t dtype, int32_t he
     const int one = dtype == NVLLM_DTYPE_FP32 ? 4 : 8;  // rows of 8 MMA columns
     const int64_t rows = int64_t(max_query_len) * group;
     w.tile_rows = rows <= one ? one : rows <= 2 * one || head_dim > 128 ? 2 * one : 4 * one;
-    w.chunk = kChunk;
-    w.min_run = 32;
+    w.chunk = kSub * subs(head_dim, w.tile_rows / one);
+    w.min_run = 512 / w.chunk;
     w.target = 148 * 3 * 5;
     return w;
 }
