@@ -83,7 +83,7 @@ struct Kv8Merge {
     int32_t seq;
     int32_t row0;
     int32_t slot;   // of the first part
-    int32_t parts;
+    int32_t parts;  // 0: nothing to merge
 };
 struct Kv8Counters {
     int32_t next;    // cursor over items x KV heads
@@ -101,8 +101,13 @@ struct Kv8Work {
     int32_t chunk;
     int32_t min_run;   // shortest run (chunks) a tile is cut into
     int32_t target;    // runs to aim for, over all KV heads
+    int32_t groups;    // > 0: one tile per sequence, cut into that many equal ranges (no plan)
+    int32_t snap;      // ranges end where sequences do: no tile is cut
     int32_t merge_grid;  // CTAs of the merge, 0: no tile is ever cut
 };
+
+// Most sequences of a call without a plan (longer batches take several).
+constexpr int kKv8SelfSeqs = 512;
 
 // Carves the workspace for a work list whose tile_rows, chunk, min_run and target
 // are set (base may be NULL to learn the size, returned in bytes).
@@ -121,6 +126,37 @@ __device__ __forceinline__ int kv8_chunk(const Kv8Item& it, int c) {
 __device__ __forceinline__ bool kv8_metadata_ok(const Kv8AttnParams& p, int q0, int qlen, int ctx) {
     return q0 >= 0 && qlen >= 0 && qlen <= ctx && qlen <= p.max_query_len &&
            ctx <= p.max_context_len && int64_t(ctx) <= int64_t(p.max_blocks) * p.a.block_size;
+}
+
+// One sequence's rows and tiles; rows < 0: metadata that contradict the bounds.
+struct Kv8Seq {
+    int first_pos;  // position of its first new row
+    int rows;       // packed rows
+    int ntiles;
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnParams& p, const Kv8Work& w, int s) {
+    const int q0 = p.cu_seqlens_q[s];
+    const int qlen = p.cu_seqlens_q[s + 1] - q0;
+    const int ctx = p.context_lens[s];
+    if (!kv8_metadata_ok(p, q0, qlen, ctx)) return {0, -1, 0};
+    const int rows = qlen * p.group;
+    return {ctx - qlen, rows, (rows + w.tile_rows - 1) / w.tile_rows};
+}
+
+// The list of tile t: chunks in all, of which sinks, and the first after them.
+struct Kv8List {
+    int n, nsink, lo;
+};
+__device__ __forceinline__ Kv8List kv8_list(const Kv8AttnParams& p, const Kv8Work& w,
+                                            const Kv8Seq& q, int t) {
+    const int r0 = t * w.tile_rows;
+    const int r1 = min(r0 + w.tile_rows, q.rows) - 1;
+    const int p0 = q.first_pos + r0 / p.group;
+    const int p1 = q.first_pos + r1 / p.group;
+    const int first = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    const int lo = first / w.chunk;
+    const int nsink = min((min(p.sinks, first) + w.chunk - 1) / w.chunk, lo);
+    return {nsink + p1 / w.chunk + 1 - lo, nsink, lo};
 }
 
 // 2^e for e in [-126, 127].

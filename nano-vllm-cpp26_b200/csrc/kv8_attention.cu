@@ -25,7 +25,8 @@
 // 8 x 8 transpose (movmatrix).
 //
 // What bounds a decode is the cache's bytes. A CTA of 4 warps takes runs of
-// chunks (kv8_plan.cu); a warp takes every fourth chunk of SUB x 16 positions and
+// chunks (kv8_plan.cu, or without a plan an equal range of a decode batch, see
+// SelfRange); a warp takes every fourth chunk of SUB x 16 positions and
 // brings them into its own two shared-memory buffers by 16-byte asynchronous
 // copies (positions that no row sees as zeros), one chunk in flight while it
 // computes the other. Of K, lane (g, t) reads the pieces t, t + 4, .. of rows g
@@ -44,6 +45,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kSub = 16;  // positions of one MMA tile
+constexpr int kSms = 148;
 
 template <typename T>
 constexpr int terms() { return sizeof(T) == 4 ? 2 : 1; }
@@ -152,6 +154,9 @@ constexpr int subs(int head_dim, int nq) {
     return nq > 2 || head_dim == 256 ? 1 : head_dim == 128 || nq == 2 ? 2 : 4;
 }
 
+// CTAs per SM, by registers and shared memory.
+constexpr int resident(int head_dim, int nq) { return head_dim * nq >= 512 || head_dim == 256 ? 2 : 3; }
+
 // One 16-position tile of K or V in shared memory: rows of HD bytes, the 16-byte
 // pieces of a 128-byte line permuted by its rows. K's reads take 8 / (HD / 16)
 // neighbouring rows' pieces at once, V's the same pieces of rows 0, 2, 4, 6: the
@@ -186,11 +191,108 @@ struct Tile {
     static constexpr size_t EXPS = RING > JOIN ? RING : JOIN;      // factors of a chunk's positions
     static constexpr size_t Q = EXPS + kWarps * 2 * SUB * 32 * 4;
     static constexpr size_t SCALE = Q + Q_WORDS * 4;
-    static constexpr size_t SMEM = SCALE + ROWS * 4;
-    static constexpr int CTAS = HD * NQ >= 512 || HD == 256 ? 2 : 3;
+    static constexpr size_t FIRST = SCALE + ROWS * 4;              // chunks before each sequence
+    static constexpr size_t SMEM = FIRST + (kKv8SelfSeqs + 1) * 4;
+    static constexpr int CTAS = resident(HD, NQ);
 };
 
-template <typename T, int kFormat, int HD, int NQ, bool kB16>
+// The range of the batch that a CTA takes when there is no plan (one tile per
+// sequence): the chunks of all sequences in a row, in w.groups equal ranges; a
+// range's CTAs, one per KV head, walk the same positions side by side, so that
+// the heads' bytes of a position, which are neighbours in memory, are read at
+// about the same time.
+struct SelfRange {
+    int x, x1;  // chunks of this CTA, from the first of all sequences
+    int s;      // sequence of x
+};
+
+// All threads: first[s] = chunks before sequence s; returns the CTA's range.
+__device__ SelfRange self_range(const Kv8AttnParams& p, const Kv8Work& w, int* first, int grp, bool lead) {
+    constexpr int PER = kKv8SelfSeqs / (kWarps * 32);
+    __shared__ int warp_sum[kWarps];
+    __shared__ int warp_some[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int n[PER], sum = 0, some = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int s = threadIdx.x * PER + i;
+        n[i] = 0;
+        if (s < p.num_seqs) {
+            const Kv8Seq q = kv8_seq(p, w, s);
+            if (q.rows < 0 && blockIdx.x == 0) raise_status(kStatusMetadata);
+            if (q.rows > 0) n[i] = kv8_list(p, w, q, 0).n;
+        }
+        sum += n[i];
+        some += n[i] > 0;
+    }
+    some = __reduce_add_sync(0xffffffffu, some);
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) {
+        warp_sum[warp] = x;
+        warp_some[warp] = some;
+    }
+    __syncthreads();
+    int before = x - sum;
+    int total = 0;
+    some = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        before += i < warp ? warp_sum[i] : 0;
+        total += warp_sum[i];
+        some += warp_some[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        first[threadIdx.x * PER + i] = before;
+        before += n[i];
+    }
+    if (threadIdx.x == 0) first[kKv8SelfSeqs] = total;
+    __syncthreads();
+    // a range is worth its partials from min_run chunks on, or a sequence of its own
+    const int groups = min(w.groups, max(max(1, some), total / w.min_run));
+    auto seq_of = [&](int at) {  // the sequence that holds chunk `at` (after empty ones)
+        int lo = 0, hi = kKv8SelfSeqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first[mid] <= at) lo = mid; else hi = mid;
+        }
+        return lo;
+    };
+    auto edge = [&](int i) {
+        const int at = int((long long)total * i / groups);
+        if (!w.snap || i == 0 || i == groups) return at;
+        const int s = seq_of(at);
+        return first[s] == at ? at : first[s + 1];
+    };
+    SelfRange r{0, 0, 0};
+    if (grp < groups) {
+        r.x = edge(grp);
+        r.x1 = edge(grp + 1);
+        if (r.x < r.x1) r.s = seq_of(r.x);
+    }
+    if (!w.snap && lead && threadIdx.x == 0) {
+        // the tile that starts in this range and goes on past it
+        Kv8Merge m{0, 0, 2 * grp + 1, 0};
+        if (r.x < r.x1 && r.x1 < total) {
+            const int s = seq_of(r.x1 - 1);
+            if (first[s] >= r.x && first[s + 1] > r.x1) {
+                m.seq = s;
+                // the range of the tile's last chunk: the first whose end is past it
+                m.parts = 2;
+                while (int((long long)total * (grp + m.parts) / groups) < first[s + 1]) ++m.parts;
+            }
+        }
+        w.merges[grp] = m;
+    }
+    return r;
+}
+
+template <typename T, int kFormat, int HD, int NQ, bool kB16, bool kSelf>
 __global__ void __launch_bounds__(kWarps * 32, Tile<T, HD, NQ>::CTAS)
 kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     using F = Frag<HD>;
@@ -217,16 +319,38 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     pdl_release();
     pdl_wait();  // the work list, the rows and the cache come from the kernels before
     const int H = p.a.num_heads;
-    const int total = w.counters->items * H;
+    const int total = kSelf ? 0 : w.counters->items * H;
+    const int grp = int(blockIdx.x) / H;
+    int* first = reinterpret_cast<int*>(smem + S::FIRST);
+    SelfRange range{0, 0, 0};
+    if constexpr (kSelf) range = self_range(p, w, first, grp, int(blockIdx.x) % H == 0);
 
     for (;;) {
-        __syncthreads();
-        if (threadIdx.x == 0) s_next = atomicAdd(&w.counters->next, 1);
-        __syncthreads();
-        const int it = s_next;
-        if (it >= total) return;
-        const Kv8Item item = w.items[it / H];
-        const int h = it % H;
+        Kv8Item item;
+        int h;
+        if constexpr (kSelf) {
+            if (range.x >= range.x1) return;
+            while (first[range.s + 1] <= range.x) ++range.s;  // sequences without rows
+            const Kv8List l = kv8_list(p, w, kv8_seq(p, w, range.s), 0);
+            item.seq = range.s;
+            item.row0 = 0;
+            item.c0 = range.x - first[range.s];
+            item.c1 = min(range.x1 - first[range.s], l.n);
+            item.nsink = l.nsink;
+            item.lo = l.lo;
+            item.slot = item.c1 - item.c0 == l.n ? -1 : 2 * grp + (item.c0 == 0 ? 1 : 0);
+            range.x = first[range.s] + item.c1;
+            h = int(blockIdx.x) % H;
+            __syncthreads();  // the buffers are free
+        } else {
+            __syncthreads();
+            if (threadIdx.x == 0) s_next = atomicAdd(&w.counters->next, 1);
+            __syncthreads();
+            const int it = s_next;
+            if (it >= total) return;
+            item = w.items[it / H];
+            h = it % H;
+        }
         const int q0 = p.cu_seqlens_q[item.seq];
         const int qlen = p.cu_seqlens_q[item.seq + 1] - q0;
         const int first_pos = p.context_lens[item.seq] - qlen;
@@ -644,32 +768,36 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
     }
 }
 
-template <typename T, int kFormat, int HD, int NQ, bool kB16>
+template <typename T, int kFormat, int HD, int NQ, bool kB16, bool kSelf>
 cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
-    auto* k = kv8_attention_kernel<T, kFormat, HD, NQ, kB16>;
+    auto* k = kv8_attention_kernel<T, kFormat, HD, NQ, kB16, kSelf>;
     constexpr size_t smem = Tile<T, HD, NQ>::SMEM;
-    static int grid_per_device[64] = {0};
+    static bool ready[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (grid_per_device[dev] == 0) {
+    if (!ready[dev]) {
         e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
         if (e != cudaSuccess) return e;
-        int sms = 0, per_sm = 0;
-        e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess) return e;
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kWarps * 32, smem);
-        if (e != cudaSuccess) return e;
-        grid_per_device[dev] = sms * std::max(per_sm, 1);
+        ready[dev] = true;
     }
-    return launch_programmatic(k, dim3(unsigned(grid_per_device[dev])), dim3(kWarps * 32), smem, st, p, w);
+    const int grid = kSelf ? w.groups * p.a.num_heads : kSms * Tile<T, HD, NQ>::CTAS;
+    return launch_programmatic(k, dim3(unsigned(grid)), dim3(kWarps * 32), smem, st, p, w);
 }
 
 template <typename T, int kFormat, int HD, int NQ>
 cudaError_t launch_blocks(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
-    return p.a.block_size % kSub == 0 ? launch_kernel<T, kFormat, HD, NQ, true>(p, w, st)
-                                        : launch_kernel<T, kFormat, HD, NQ, false>(p, w, st);
+    const bool b16 = p.a.block_size % kSub == 0;
+    if (w.groups > 0) {
+        return b16 ? launch_kernel<T, kFormat, HD, NQ, true, true>(p, w, st)
+                   : launch_kernel<T, kFormat, HD, NQ, false, true>(p, w, st);
+    }
+    if constexpr (NQ == 4 || HD == 256) {  // several tiles per sequence: the largest ones
+        return b16 ? launch_kernel<T, kFormat, HD, NQ, true, false>(p, w, st)
+                   : launch_kernel<T, kFormat, HD, NQ, false, false>(p, w, st);
+    }
+    return cudaErrorInvalidValue;
 }
 
 template <typename T, int kFormat, int HD>
@@ -701,15 +829,36 @@ cudaError_t launch_type(const Kv8AttnParams& p, const Kv8Work& w, int32_t format
                                     : launch_hd<T, NVLLM_KV8_INT8>(p, w, st);
 }
 
-// The work list's shape for these rows.
-Kv8Work work_for(int32_t max_query_len, int32_t group, int32_t dtype, int32_t head_dim) {
+// Columns (rows of one term) of 8-column MMA tiles for this many packed rows.
+int columns_for(int64_t rows, int one, int head_dim) {
+    return rows <= one ? 1 : rows <= 2 * one || head_dim > 128 ? 2 : 4;
+}
+
+// Rows of one 8-column tile.
+int rows_of_tile(int32_t dtype) { return dtype == NVLLM_DTYPE_FP32 ? 4 : 8; }
+
+// The work list of a batch whose sequences are one tile each.
+Kv8Work self_work(int nq, int32_t dtype, int32_t max_context_len, const ArenaGeom& g) {
     Kv8Work w{};
-    const int one = dtype == NVLLM_DTYPE_FP32 ? 4 : 8;  // rows of 8 MMA columns
+    w.tile_rows = nq * rows_of_tile(dtype);
+    w.chunk = kSub * subs(g.head_dim, nq);
+    w.groups = std::max(1, kSms * resident(g.head_dim, nq) / g.num_heads);
+    w.min_run = std::max(1, 256 / w.chunk);
+    w.snap = max_context_len <= 512;
+    return w;
+}
+
+Kv8Work work_for(int32_t max_query_len, int32_t max_context_len, int32_t group, int32_t dtype,
+                 const ArenaGeom& g) {
+    const int one = rows_of_tile(dtype);
     const int64_t rows = int64_t(max_query_len) * group;
-    w.tile_rows = rows <= one ? one : rows <= 2 * one || head_dim > 128 ? 2 * one : 4 * one;
-    w.chunk = kSub * subs(head_dim, w.tile_rows / one);
+    const int nq = columns_for(rows, one, g.head_dim);
+    if (rows <= nq * one) return self_work(nq, dtype, max_context_len, g);
+    Kv8Work w{};
+    w.tile_rows = nq * one;
+    w.chunk = kSub * subs(g.head_dim, nq);
     w.min_run = 512 / w.chunk;
-    w.target = 148 * 3 * 5;
+    w.target = kSms * resident(g.head_dim, nq) * 5;
     return w;
 }
 
@@ -717,33 +866,52 @@ Kv8Work work_for(int32_t max_query_len, int32_t group, int32_t dtype, int32_t he
 
 size_t kv8_attention_workspace(int32_t num_seqs, int32_t max_query_len, int32_t max_context_len,
                                int32_t num_query_heads, const ArenaGeom& g) {
+    // of the call itself and of every smaller one: a workspace serves them all
     const int group = num_query_heads / g.num_heads;
     size_t n = 0;
     for (int32_t dtype : {NVLLM_DTYPE_FP32, NVLLM_DTYPE_BF16}) {
-        Kv8Work w = work_for(max_query_len, group, dtype, g.head_dim);
+        Kv8Work w = work_for(max_query_len, max_context_len, group, dtype, g);
         n = std::max(n, kv8_work_layout(w, nullptr, num_seqs, max_query_len, max_context_len, group, g));
+        const int nq = w.tile_rows / rows_of_tile(dtype);
+        for (int q = 1; q <= nq; q *= 2) {
+            Kv8Work self = self_work(q, dtype, max_context_len, g);
+            n = std::max(n, kv8_work_layout(self, nullptr, num_seqs, 1, max_context_len, 1, g));
+        }
     }
     return n;
 }
 
-cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int32_t dtype, int32_t format,
+cudaError_t launch_kv8_attention(const Kv8AttnParams& all, int32_t dtype, int32_t format,
                                  void* workspace, cudaStream_t stream) {
-    Kv8Work w = work_for(p.max_query_len, p.group, dtype, p.a.head_dim);
     ArenaGeom g{};
-    g.num_heads = p.a.num_heads;
-    g.head_dim = p.a.head_dim;
-    kv8_work_layout(w, static_cast<unsigned char*>(workspace), p.num_seqs, p.max_query_len,
-                    p.max_context_len, p.group, g);
-    cudaError_t e = launch_kv8_plan(p, w, stream);
-    if (e != cudaSuccess) return e;
-    switch (dtype) {
-        case NVLLM_DTYPE_FP32: e = launch_type<float>(p, w, format, stream); break;
-        case NVLLM_DTYPE_BF16: e = launch_type<__nv_bfloat16>(p, w, format, stream); break;
-        case NVLLM_DTYPE_FP16: e = launch_type<__half>(p, w, format, stream); break;
-        default: return cudaErrorInvalidValue;
+    g.num_heads = all.a.num_heads;
+    g.head_dim = all.a.head_dim;
+    Kv8Work w = work_for(all.max_query_len, all.max_context_len, all.group, dtype, g);
+    // without a plan a call counts at most kKv8SelfSeqs sequences itself
+    const int step = w.groups > 0 ? kKv8SelfSeqs : all.num_seqs;
+    for (int s = 0; s < all.num_seqs; s += step) {
+        Kv8AttnParams p = all;
+        p.num_seqs = std::min(step, all.num_seqs - s);
+        p.block_tables += int64_t(s) * p.max_blocks;
+        p.cu_seqlens_q += s;
+        p.context_lens += s;
+        kv8_work_layout(w, static_cast<unsigned char*>(workspace), p.num_seqs, p.max_query_len,
+                        p.max_context_len, p.group, g);
+        cudaError_t e = w.groups > 0 ? cudaSuccess : launch_kv8_plan(p, w, stream);
+        if (e != cudaSuccess) return e;
+        switch (dtype) {
+            case NVLLM_DTYPE_FP32: e = launch_type<float>(p, w, format, stream); break;
+            case NVLLM_DTYPE_BF16: e = launch_type<__nv_bfloat16>(p, w, format, stream); break;
+            case NVLLM_DTYPE_FP16: e = launch_type<__half>(p, w, format, stream); break;
+            default: return cudaErrorInvalidValue;
+        }
+        if (e != cudaSuccess) return e;
+        if (w.merge_grid > 0) {
+            e = launch_kv8_merge(p, w, dtype, stream);
+            if (e != cudaSuccess) return e;
+        }
     }
-    if (e != cudaSuccess || w.merge_grid == 0) return e;
-    return launch_kv8_merge(p, w, dtype, stream);
+    return cudaSuccess;
 }
 
 }  // namespace nvllm

@@ -18,38 +18,6 @@ constexpr int kPlanThreads = 1024;
 
 size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
 
-// One sequence's rows and tiles; rows < 0: metadata that contradict the bounds.
-struct Kv8Seq {
-    int first_pos;  // position of its first new row
-    int rows;       // packed rows
-    int ntiles;
-};
-
-__device__ __forceinline__ Kv8Seq load_seq(const Kv8AttnParams& p, const Kv8Work& w, int s) {
-    const int q0 = p.cu_seqlens_q[s];
-    const int qlen = p.cu_seqlens_q[s + 1] - q0;
-    const int ctx = p.context_lens[s];
-    if (!kv8_metadata_ok(p, q0, qlen, ctx)) return {0, -1, 0};
-    const int rows = qlen * p.group;
-    return {ctx - qlen, rows, (rows + w.tile_rows - 1) / w.tile_rows};
-}
-
-// The list of tile t: chunks in all, of which sinks, and the first after them.
-struct Kv8List {
-    int n, nsink, lo;
-};
-__device__ __forceinline__ Kv8List tile_list(const Kv8AttnParams& p, const Kv8Work& w,
-                                             const Kv8Seq& q, int t) {
-    const int r0 = t * w.tile_rows;
-    const int r1 = min(r0 + w.tile_rows, q.rows) - 1;
-    const int p0 = q.first_pos + r0 / p.group;
-    const int p1 = q.first_pos + r1 / p.group;
-    const int first = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
-    const int lo = first / w.chunk;
-    const int nsink = min((min(p.sinks, first) + w.chunk - 1) / w.chunk, lo);
-    return {nsink + p1 / w.chunk + 1 - lo, nsink, lo};
-}
-
 // kWide: a warp per sequence, its lanes over the tiles; else a thread per sequence.
 template <bool kWide>
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnParams p, const Kv8Work w) {
@@ -69,9 +37,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
     __syncthreads();
     long long mine = 0;
     for (int s = me; s < p.num_seqs; s += kSeqs) {
-        const Kv8Seq q = load_seq(p, w, s);
+        const Kv8Seq q = kv8_seq(p, w, s);
         if (q.rows < 0 && t0 == 0) raise_status(kStatusMetadata);
-        for (int t = t0; t < q.ntiles; t += kStep) mine += tile_list(p, w, q, t).n;
+        for (int t = t0; t < q.ntiles; t += kStep) mine += kv8_list(p, w, q, t).n;
     }
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0 && mine) atomicAdd(&total, (unsigned long long)mine);
@@ -81,11 +49,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
     // the longest lists, those of a sequence's last tiles, go out first
     for (int base = 0; base < p.num_seqs; base += kSeqs) {
         const int s = base + me;
-        const Kv8Seq q = s < p.num_seqs ? load_seq(p, w, s) : Kv8Seq{0, 0, 0};
+        const Kv8Seq q = s < p.num_seqs ? kv8_seq(p, w, s) : Kv8Seq{0, 0, 0};
         for (int i = 0;; i += kStep) {
             const int t = q.ntiles - 1 - i - t0;
             if (!__any_sync(0xffffffffu, t >= 0)) break;
-            const Kv8List l = t >= 0 ? tile_list(p, w, q, t) : Kv8List{0, 0, 0};
+            const Kv8List l = t >= 0 ? kv8_list(p, w, q, t) : Kv8List{0, 0, 0};
             const int parts = t < 0 ? 0 : l.n > run ? (l.n + run - 1) / run : 1;
             const int slots = parts > 1 ? parts : 0;
             // this lane's places: an inclusive scan of both counts in one word
@@ -107,12 +75,35 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
             bi = __shfl_sync(0xffffffffu, bi, 31) + int(x & 0xffffffff) - parts;
             bs = __shfl_sync(0xffffffffu, bs, 31) + int(x >> 32) - slots;
             bm = __shfl_sync(0xffffffffu, bm, 31) + __popc(cut & ((1u << lane) - 1));
-            for (int k = 0; k < parts; ++k) {
+            // a tile in many parts is written by the warp together, the others by their lanes
+            constexpr int kFew = 8;
+            for (int k = 0; k < parts && parts <= kFew; ++k) {
                 w.items[bi + k] = Kv8Item{s, t * w.tile_rows, int((long long)l.n * k / parts),
                                           int((long long)l.n * (k + 1) / parts), l.nsink, l.lo,
                                           parts > 1 ? bs + k : -1, 0};
             }
             if (slots > 0) w.merges[bm] = Kv8Merge{s, t * w.tile_rows, bs, parts};
+            for (unsigned left = __ballot_sync(0xffffffffu, parts > kFew); left; left &= left - 1) {
+                const int from = __ffs(left) - 1;
+                const int n = __shfl_sync(0xffffffffu, parts, from);
+                const int i0 = __shfl_sync(0xffffffffu, bi, from);
+                const int s0 = __shfl_sync(0xffffffffu, bs, from);
+                const long long len = __shfl_sync(0xffffffffu, l.n, from);
+                Kv8Item item{__shfl_sync(0xffffffffu, s, from),
+                             __shfl_sync(0xffffffffu, t, from) * w.tile_rows,
+                             0,
+                             0,
+                             __shfl_sync(0xffffffffu, l.nsink, from),
+                             __shfl_sync(0xffffffffu, l.lo, from),
+                             0,
+                             0};
+                for (int k = lane; k < n; k += 32) {
+                    item.c0 = int(len * k / n);
+                    item.c1 = int(len * (k + 1) / n);
+                    item.slot = s0 + k;
+                    w.items[i0 + k] = item;
+                }
+            }
         }
     }
     __syncthreads();
@@ -128,15 +119,22 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p, c
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int H = p.a.num_heads;
-    const long long total = (long long)w.counters->merges * H * w.tile_rows;
+    // without a plan every range has an entry; a range's partials are its first
+    // tile's, which began in an earlier range, then its last one's
+    const long long merges = w.groups > 0 ? w.groups : w.counters->merges;
+    const long long total = merges * H * w.tile_rows;
     for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += gridDim.x * 8ll) {
         const int r = int(i % w.tile_rows);
         const int h = int(i / w.tile_rows % H);
         const Kv8Merge m = w.merges[i / w.tile_rows / H];
+        if (m.parts == 0) continue;
         const int q0 = p.cu_seqlens_q[m.seq];
         const int row = m.row0 + r;
         if (row >= (p.cu_seqlens_q[m.seq + 1] - q0) * p.group) continue;
-        const auto at = [&](int k) { return (int64_t(m.slot + k) * H + h) * w.tile_rows + r; };
+        const auto at = [&](int k) { 
+            const int slot = m.slot + (w.groups > 0 && k > 0 ? 2 * k - 1 : k);
+            return (int64_t(slot) * H + h) * w.tile_rows + r;
+        };
         float M = -INFINITY;
         for (int k = lane; k < m.parts; k += 32) M = fmaxf(M, __ldcg(&w.ml[at(k)].x));
         M = warp_max_xor(M, 32);
@@ -198,7 +196,12 @@ size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_
     const int64_t chunks = (int64_t(max_context_len) + w.chunk - 1) / w.chunk + 2;
     const bool cut = chunks > w.min_run;
     const int64_t parts = cut ? (chunks + w.min_run - 1) / w.min_run : 1;
-    const int64_t slots = cut ? std::min<int64_t>(2 * int64_t(w.target) / g.num_heads + 1, units * parts) : 0;
+    int64_t slots = cut ? std::min<int64_t>(2 * int64_t(w.target) / g.num_heads + 1, units * parts) : 0;
+    int64_t merges = slots;
+    if (w.groups > 0) {
+        merges = w.snap ? 0 : w.groups;
+        slots = 2 * merges;
+    }
     size_t off = 0;
     auto take = [&](size_t bytes) {
         unsigned char* at = base + off;
@@ -206,11 +209,11 @@ size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_
         return at;
     };
     w.counters = reinterpret_cast<Kv8Counters*>(take(sizeof(Kv8Counters)));
-    w.items = reinterpret_cast<Kv8Item*>(take(size_t(units + slots) * sizeof(Kv8Item)));
-    w.merges = reinterpret_cast<Kv8Merge*>(take(size_t(slots) * sizeof(Kv8Merge)));
+    w.items = reinterpret_cast<Kv8Item*>(take(size_t(w.groups > 0 ? 0 : units + slots) * sizeof(Kv8Item)));
+    w.merges = reinterpret_cast<Kv8Merge*>(take(size_t(merges) * sizeof(Kv8Merge)));
     w.ml = reinterpret_cast<float2*>(take(size_t(slots) * g.num_heads * w.tile_rows * sizeof(float2)));
     w.acc = reinterpret_cast<float*>(take(size_t(slots) * g.num_heads * w.tile_rows * g.head_dim * sizeof(float)));
-    const int64_t rows = std::min<int64_t>(units, slots) * g.num_heads * w.tile_rows;
+    const int64_t rows = std::min<int64_t>(units, merges) * g.num_heads * w.tile_rows;
     w.merge_grid = int32_t(std::min<int64_t>((rows + 7) / 8, 148 * 4));
     return off;
 }
