@@ -21,6 +21,7 @@ enum : uint32_t {
     kStatusInPrefill = 1u << 13,
     kStatusInHeadGather = 1u << 14,
     kStatusInHeadSplit = 1u << 15,  // the head split's wait for every rank's rows
+    kStatusInKv8Tc = 1u << 16,
 };
 
 extern __device__ uint32_t g_status;

@@ -211,4 +211,10 @@ size_t kv8_attention_workspace(int32_t num_seqs, int32_t max_query_len, int32_t 
 cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int32_t dtype, int32_t format,
                                  void* workspace, cudaStream_t stream);
 
+// The kernel for many rows per KV head (kv8_attention_tc.cu).
+bool kv8_tc_supported(int32_t dtype, int32_t head_dim);
+Kv8Work kv8_tc_work();
+cudaError_t launch_kv8_tc(const Kv8AttnParams& p, const Kv8Work& w, int32_t dtype, int32_t format,
+                          cudaStream_t stream);
+
 }  // namespace nvllm

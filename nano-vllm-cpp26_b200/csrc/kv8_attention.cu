@@ -793,7 +793,9 @@ cudaError_t launch_blocks(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t
         return b16 ? launch_kernel<T, kFormat, HD, NQ, true, true>(p, w, st)
                    : launch_kernel<T, kFormat, HD, NQ, false, true>(p, w, st);
     }
-    if constexpr (NQ == 4 || HD == 256) {  // several tiles per sequence: the largest ones
+    // several tiles per sequence: the largest ones, of what the tensor-memory kernel
+    // does not take
+    if constexpr ((NQ == 4 && (HD == 32 || sizeof(T) == 4)) || (NQ == 2 && HD == 256)) {
         return b16 ? launch_kernel<T, kFormat, HD, NQ, true, false>(p, w, st)
                    : launch_kernel<T, kFormat, HD, NQ, false, false>(p, w, st);
     }
@@ -854,6 +856,7 @@ Kv8Work work_for(int32_t max_query_len, int32_t max_context_len, int32_t group, 
     const int64_t rows = int64_t(max_query_len) * group;
     const int nq = columns_for(rows, one, g.head_dim);
     if (rows <= nq * one) return self_work(nq, dtype, max_context_len, g);
+    if (kv8_tc_supported(dtype, g.head_dim)) return kv8_tc_work();
     Kv8Work w{};
     w.tile_rows = nq * one;
     w.chunk = kSub * subs(g.head_dim, nq);
@@ -872,8 +875,7 @@ size_t kv8_attention_workspace(int32_t num_seqs, int32_t max_query_len, int32_t 
     for (int32_t dtype : {NVLLM_DTYPE_FP32, NVLLM_DTYPE_BF16}) {
         Kv8Work w = work_for(max_query_len, max_context_len, group, dtype, g);
         n = std::max(n, kv8_work_layout(w, nullptr, num_seqs, max_query_len, max_context_len, group, g));
-        const int nq = w.tile_rows / rows_of_tile(dtype);
-        for (int q = 1; q <= nq; q *= 2) {
+        for (int q = 1; q <= columns_for(int64_t(max_query_len) * group, rows_of_tile(dtype), g.head_dim); q *= 2) {
             Kv8Work self = self_work(q, dtype, max_context_len, g);
             n = std::max(n, kv8_work_layout(self, nullptr, num_seqs, 1, max_context_len, 1, g));
         }
@@ -899,11 +901,14 @@ cudaError_t launch_kv8_attention(const Kv8AttnParams& all, int32_t dtype, int32_
                         p.max_context_len, p.group, g);
         cudaError_t e = w.groups > 0 ? cudaSuccess : launch_kv8_plan(p, w, stream);
         if (e != cudaSuccess) return e;
-        switch (dtype) {
-            case NVLLM_DTYPE_FP32: e = launch_type<float>(p, w, format, stream); break;
-            case NVLLM_DTYPE_BF16: e = launch_type<__nv_bfloat16>(p, w, format, stream); break;
-            case NVLLM_DTYPE_FP16: e = launch_type<__half>(p, w, format, stream); break;
-            default: return cudaErrorInvalidValue;
+        if (w.groups == 0 && kv8_tc_supported(dtype, g.head_dim)) {
+            e = launch_kv8_tc(p, w, dtype, format, stream);
+        } else if (dtype == NVLLM_DTYPE_FP32) {
+            e = launch_type<float>(p, w, format, stream);
+        } else if (dtype == NVLLM_DTYPE_BF16) {
+            e = launch_type<__nv_bfloat16>(p, w, format, stream);
+        } else {
+            e = launch_type<__half>(p, w, format, stream);
         }
         if (e != cudaSuccess) return e;
         if (w.merge_grid > 0) {

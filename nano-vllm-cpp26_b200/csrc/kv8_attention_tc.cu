@@ -1,0 +1,783 @@
+// Attention over the 8-bit paged cache for many rows per KV head (prompts and
+// chunks), on tcgen05 with accumulators in tensor memory; bf16 and fp16 rows,
+// head_dim 64 and 128, any block size.
+//
+// A tile is 256 packed rows (kv8.cuh) of one sequence and KV head, two halves of
+// 128; keys come in tiles of 64. With q' = q scaled by a power of two to [1, 2)
+// per row, codes c_j, d_j and exponents a_j, b_j of K and V, and A the largest a_j
+// of a key tile (U = 7 for E4M3, 5 for INT8):
+//   K'_j = c_j 2^(a_j - A + U)                 in fp16
+//   S = q' . K'_j,  x_j = S 2^(A - U) qs       log2-domain score
+//   m = running max of x_j,  P_j = 2^(x_j - m)   in bf16
+//   acc += sum_j P_j V_j,  l += sum_j P_j,  o = acc / l     V_j = d_j 2^(b_j) in bf16
+// The exponents cost nothing per score: they are folded into the operands while
+// codes become 16-bit floats, K's against the tile's largest, which is one more
+// factor of the row's scale. V is exact in bf16 whatever its exponent; K' in fp16
+// is exact for rows within 2^22 of the tile's largest (2^29 for INT8) and beyond
+// that off by 2^-36 of the largest. P is rounded to bf16, half a step of which is
+// the output's own; for fp16 rows, whose step is finer, P is two bf16 terms.
+//
+// One CTA per SM, 16 warps in 4 warpgroups:
+//   warps 0-3, 4-7  softmax of the tile's first and second 128 rows: a thread owns
+//                   a row and its TMEM lane. Reads S, masks ragged tiles, P goes
+//                   back over S as the next product's A operand; O is rescaled
+//                   only when m moves by more than kMargin (rarely).
+//   warp 12         MMAs, one lane: S(n+1) of both halves is queued while the
+//                   softmax works on S(n), then O(n) += P(n) V(n) of each half.
+//                   Its warpgroup (three more warps that do nothing) gives its
+//                   registers to the softmax.
+//   warps 8-11      converters: 16 codes per thread from the arenas to registers a
+//                   tile ahead (block ids two ahead), then as fp16 into a ring of
+//                   three stages in the MMA's 128-byte swizzle; rows that no query
+//                   of the tile sees become zeros.
+// TMEM (512 columns): S of half i, buffer b at 128 i + 64 b, O of half i at 256 +
+// 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
+// special function units, as many as the products take on the tensor cores at
+// head_dim 128.
+// Every wait is bounded; on a timeout the CTA records NVLLM_ERR_TIMEOUT, lets its
+// MMAs finish and frees its TMEM.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv8.cuh"
+#include "tcgen05.cuh"
+
+namespace nvllm {
+
+namespace {
+
+constexpr int kHalf = 128;           // rows of a half (TMEM lanes)
+constexpr int kRows = 2 * kHalf;     // rows of a tile
+constexpr int kKeys = 64;            // keys of a key tile
+constexpr int kStages = 3;
+constexpr int kConvWarp0 = 8;
+constexpr int kConvThreads = 128;
+constexpr int kMmaWarp = 12;
+constexpr int kThreads = 512;
+constexpr int kItemReaders = kMmaWarp;  // every working warp but the first converter
+// Registers a thread: 128 at launch (65536 / 512). The MMA's warpgroup falls to 40,
+// which frees 88 x 128; the two softmax warpgroups rise to 160 and the converters
+// to 152, which takes (32 + 32 + 24) x 128.
+constexpr int kMmaRegs = 40;
+constexpr int kSoftmaxRegs = 160;
+constexpr int kConvRegs = 152;
+static_assert(2 * kSoftmaxRegs + kConvRegs + kMmaRegs <= 4 * 128, "register split");
+constexpr uint32_t kTmemCols = 512;
+constexpr int kSms = 148;
+constexpr float kMargin = 8.0f;
+
+template <int kFormat>
+constexpr int kUp = kFormat == NVLLM_KV8_E4M3 ? 7 : 5;
+
+// Instruction descriptors for kind::f16 with fp32 accumulation: fp16 or bf16 A and B.
+constexpr uint32_t idesc(int M, int N, bool bf16, bool b_mn) {
+    return (1u << 4)                   // D format: f32
+           | (uint32_t(bf16) << 7)     // A format
+           | (uint32_t(bf16) << 10)    // B format
+           | (uint32_t(b_mn) << 16)    // B major
+           | (uint32_t(N >> 3) << 17)  // N / 8
+           | (uint32_t(M >> 4) << 24); // M / 16
+}
+
+struct Control {
+    uint64_t kc_full[kStages];  // K' of a stage written (every converter thread)
+    uint64_t vc_full[kStages];  // V' of a stage written
+    uint64_t st_free[kStages];  // O of the stage's key tile complete
+    uint64_t s_full[2][2];      // [half][buffer]: S complete
+    uint64_t p_full[2][2];      // P written, O rescaled if need be (128 arrivals)
+    uint64_t o_full[2][2];      // O of that key tile complete
+    uint64_t drain;
+    uint64_t item_full[2];      // two-slot queue of work items
+    uint64_t item_free[2];
+    uint64_t q_full;            // Q of the item written (256 arrivals)
+    int32_t top[kStages];       // A of the stage's key tile
+    uint32_t tmem_base;
+    int32_t items[2];
+    int32_t abort;
+};
+
+template <int HD>
+struct Shape {
+    static constexpr uint32_t ATOM = kKeys * 128;           // 64 keys x 64 dims of K' or V'
+    static constexpr uint32_t TILE = ATOM * (HD / 64);
+    static constexpr uint32_t STAGE = 2 * TILE;
+    static constexpr uint32_t Q_ATOM = kHalf * 128;         // 128 rows x 64 dims
+    static constexpr uint32_t Q_HALF = Q_ATOM * (HD / 64);
+    static constexpr uint32_t OFF_Q = 0;
+    static constexpr uint32_t OFF_KV = 2 * Q_HALF;
+    static constexpr uint32_t OFF_CTL = OFF_KV + kStages * STAGE;
+    static constexpr uint32_t SMEM = OFF_CTL + 512 + 1024;  // + control block + alignment slack
+    static_assert(SMEM <= 227u * 1024u, "shared memory");
+    static_assert(sizeof(Control) <= 512, "control block");
+    static constexpr int PIECES = HD / 16;                     // 16-code pieces of a row
+    static constexpr int STEP = kConvThreads / PIECES;         // rows converted at once
+    static constexpr int COPIES = kKeys / STEP;                // per thread and tensor
+};
+
+// Bounded wait that also gives up once another role has aborted.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile int32_t*>(&ctl->abort)) return false;
+        if (global_ns() - t0 > kWaitLimitNs) {
+            raise_status(kStatusTimeout | kStatusInKv8Tc);
+            atomicExch(&ctl->abort, 1);
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ float ex2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// What pack_bf16 left of a and b, as bf16.
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t h) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h));
+    return pack_bf16(a - f.x, b - f.y);
+}
+
+// 2^e as an fp16 pair, e <= 15 (below 2^-24: 0).
+__device__ __forceinline__ __half2 half_power(int e) {
+    return __float2half2_rn(exp2_int(max(e, -30)));
+}
+
+// Four codes times f (a power of two) -> two fp16 pairs, in order.
+template <int kFormat>
+__device__ __forceinline__ void scaled_half4(uint32_t w, __half2 f, uint32_t& a, uint32_t& b) {
+    __half2 x, y;
+    if constexpr (kFormat == NVLLM_KV8_E4M3) {
+        uint32_t lo, hi;
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+        x = __hmul2(*reinterpret_cast<__half2*>(&lo), f);
+        y = __hmul2(*reinterpret_cast<__half2*>(&hi), f);
+    } else {
+        // (1024 + u) - 1152 = code for u = code + 128: exact, then the factor
+        const uint32_t u = w ^ 0x80808080u;
+        const __half2 c = __half2half2(__ushort_as_half(0x6480));
+        uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+        x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), c), f);
+        y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), c), f);
+    }
+    a = *reinterpret_cast<const uint32_t*>(&x);
+    b = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Four codes times 2^e -> the bf16 pairs (0, 2) and (1, 3): bytes that are two
+// apart land in a word's halves without a byte shuffle, and the epilogue knows.
+// E4M3: sign, exponent and mantissa bits moved into a bf16 are code * 2^-120 (its
+// subnormals too), so f = 2^(e + 120). INT8: 128 + the low seven bits as a bf16,
+// less 128, or 256 where the sign bit is set; f = 2^e.
+template <int kFormat>
+__device__ __forceinline__ void scaled_bf16x4(uint32_t w, __nv_bfloat162 f, uint32_t& even, uint32_t& odd) {
+    __nv_bfloat162 x, y;
+    if constexpr (kFormat == NVLLM_KV8_E4M3) {
+        uint32_t lo = ((w & 0x007F007Fu) << 4) | ((w & 0x00800080u) << 8);
+        uint32_t hi = ((w & 0x7F007F00u) >> 4) | (w & 0x80008000u);
+        x = *reinterpret_cast<__nv_bfloat162*>(&lo);
+        y = *reinterpret_cast<__nv_bfloat162*>(&hi);
+    } else {
+        const uint32_t v = w >> 8;
+        uint32_t a = (w & 0x007F007Fu) | 0x43004300u, b = (w & 0x00800080u) | 0xC300C300u;
+        uint32_t c = (v & 0x007F007Fu) | 0x43004300u, d = (v & 0x00800080u) | 0xC300C300u;
+        x = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        y = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&c), *reinterpret_cast<__nv_bfloat162*>(&d));
+    }
+    x = __hmul2(x, f);
+    y = __hmul2(y, f);
+    even = *reinterpret_cast<const uint32_t*>(&x);
+    odd = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+template <typename T, int kFormat, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
+    using S = Shape<HD>;
+    constexpr int U = kUp<kFormat>;
+    constexpr int NP = std::is_same_v<T, __half> ? 2 : 1;  // terms of P
+    constexpr uint32_t kIdescS = idesc(kHalf, kKeys, false, false);
+    constexpr uint32_t kIdescO = idesc(kHalf, HD, true, true);
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* sQ = base + S::OFF_Q;
+    unsigned char* sKV = base + S::OFF_KV;
+    Control* ctl = reinterpret_cast<Control*>(base + S::OFF_CTL);
+    const int tid = threadIdx.x;
+    const int warp = tid >> 5;
+    const int lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&ctl->kc_full[i], kConvThreads);
+            mbar_init(&ctl->vc_full[i], kConvThreads);
+            mbar_init(&ctl->st_free[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&ctl->s_full[i][b], 1);
+                mbar_init(&ctl->p_full[i][b], kHalf);
+                mbar_init(&ctl->o_full[i][b], 1);
+            }
+            mbar_init(&ctl->item_full[i], 1);
+            mbar_init(&ctl->item_free[i], kItemReaders);
+        }
+        mbar_init(&ctl->drain, 1);
+        mbar_init(&ctl->q_full, kRows);
+        ctl->abort = 0;
+    }
+    fence_barrier_init();
+    if (warp == kMmaWarp) {
+        tc::tmem_alloc(&ctl->tmem_base, kTmemCols);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = ctl->tmem_base;
+    pdl_release();
+    pdl_wait();  // the work list, the rows and the cache come from the kernels before
+
+    const int H = p.a.num_heads;
+    const int total = w.counters->items * H;
+    uint32_t seq = 0;          // key tiles of this CTA so far, and of the first half
+    uint32_t seq1 = 0;         // and of the second half
+    bool issued_mma = false;   // MMA warp
+
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl));
+    };
+    // Work items: the first converter warp takes each from the global cursor and
+    // publishes it in queue slot j % 2; every other warp reads the items in order
+    // and frees the slot. -1 ends the loop. No role waits for the others at an
+    // item's end.
+    auto publish = [&](uint32_t j, int it) -> bool {
+        const uint32_t slot = j & 1u;
+        if (j >= 2 && !wait_or_abort(&ctl->item_free[slot], ((j >> 1) - 1) & 1u, ctl)) return false;
+        ctl->items[slot] = it;
+        mbar_arrive(&ctl->item_full[slot]);
+        return true;
+    };
+    auto take = [&](uint32_t j) -> int {
+        const uint32_t slot = j & 1u;
+        if (!wait_all(&ctl->item_full[slot], (j >> 1) & 1u)) return -1;
+        const int it = *reinterpret_cast<volatile int32_t*>(&ctl->items[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->item_free[slot]);
+        return it;
+    };
+
+    auto next_item = [&](uint32_t j) -> int {
+        int it = -1;
+        if (warp == kConvWarp0) {
+            if (lane == 0) {
+                if (!*reinterpret_cast<volatile int32_t*>(&ctl->abort)) {
+                    it = atomicAdd(&w.counters->next, 1);
+                    if (it >= total) it = -1;
+                }
+                if (!publish(j, it)) it = -1;
+            }
+            it = __shfl_sync(0xffffffffu, it, 0);
+        } else {
+            it = take(j);
+        }
+        return *reinterpret_cast<volatile int32_t*>(&ctl->abort) ? -1 : it;
+    };
+    struct Job {
+        Kv8Item item;
+        int h, q0, first_pos, nrows, ntiles, halves, pos_lo, pos_hi;
+    };
+    auto job_of = [&](int it) -> Job {
+        Job x;
+        x.item = w.items[it / H];
+        x.h = it % H;
+        x.q0 = p.cu_seqlens_q[x.item.seq];
+        const int qlen = p.cu_seqlens_q[x.item.seq + 1] - x.q0;
+        x.first_pos = p.context_lens[x.item.seq] - qlen;
+        x.nrows = min(kRows, qlen * p.group - x.item.row0);
+        x.ntiles = x.item.c1 - x.item.c0;
+        x.halves = x.nrows > kHalf ? 2 : 1;
+        x.pos_lo = x.first_pos + x.item.row0 / p.group;
+        x.pos_hi = x.first_pos + (x.item.row0 + x.nrows - 1) / p.group;
+        return x;
+    };
+    auto done = [&](const Job& x) {
+        seq += x.ntiles;
+        if (x.halves == 2) seq1 += x.ntiles;
+    };
+
+    if (warp < kConvWarp0) {
+        // ---------------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        for (uint32_t j = 0;; ++j) {
+            const int it = next_item(j);
+            if (it < 0) break;
+            const Job job = job_of(it);
+            const Kv8Item& item = job.item;
+            const int h = job.h, q0 = job.q0, first_pos = job.first_pos, nrows = job.nrows;
+            const int ntiles = job.ntiles, halves = job.halves, pos_lo = job.pos_lo, pos_hi = job.pos_hi;
+            const uint32_t n0 = seq;
+            const int half = warp >> 2;
+            const uint32_t hn0 = half ? seq1 : seq;
+            const int r = tid - half * kHalf;              // row of the half, TMEM lane
+            const int row = item.row0 + half * kHalf + r;  // packed row
+            const bool live = half * kHalf + r < nrows;
+            const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+            const uint32_t tO = tmem + 256u + 128u * half + lane_off;
+            float qs = 0.f;
+            if (half < halves) {
+                // Q's row as fp16, scaled to [1, 2); this half's earlier S all completed
+                constexpr int N = HD / 8;  // 16-byte pieces of the row
+                uint4 raw[N];
+                const uint4* src = reinterpret_cast<const uint4*>(
+                    static_cast<const T*>(p.q) + int64_t(q0 + row / p.group) * p.q_stride +
+                    int64_t(h * p.group + row % p.group) * HD);
+                float a = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (live) raw[i] = __ldg(src + i);
+                    const T* v = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(to_float(v[k])));
+                }
+                const int e = min(max(int(__float_as_uint(a) >> 23) - 127, -126), 126);
+                const float inv = exp2_int(-e);
+                qs = exp2_int(e) * p.qk_scale_log2;
+                unsigned char* dst = sQ + half * S::Q_HALF + r * 128;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const T* v = reinterpret_cast<const T*>(&raw[i]);
+                    uint4 o;
+                    o.x = pack_half(to_float(v[0]) * inv, to_float(v[1]) * inv);
+                    o.y = pack_half(to_float(v[2]) * inv, to_float(v[3]) * inv);
+                    o.z = pack_half(to_float(v[4]) * inv, to_float(v[5]) * inv);
+                    o.w = pack_half(to_float(v[6]) * inv, to_float(v[7]) * inv);
+                    *reinterpret_cast<uint4*>(dst + (i >> 3) * S::Q_ATOM + ((i & 7) ^ (r & 7)) * 16) = o;
+                }
+                tc::fence_async_smem();
+            }
+            mbar_arrive(&ctl->q_full);
+            const int pos = first_pos + (item.row0 + min(half * kHalf + r, nrows - 1)) / p.group;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int t = 0; half < halves && t < ntiles; ++t) {
+                const uint32_t n = n0 + t;
+                const uint32_t hn = hn0 + t;
+                const uint32_t b = hn & 1u;
+                // (the stage's own barrier orders its exponents)
+                if (!wait_all(&ctl->kc_full[n % kStages], (n / kStages) & 1u) ||
+                    !wait_all(&ctl->s_full[half][b], (hn >> 1) & 1u)) {
+                    ok = false;
+                    break;
+                }
+                const int A = *reinterpret_cast<const volatile int32_t*>(&ctl->top[n % kStages]);
+                tc::fence_after_sync();
+                const uint32_t tS = tmem + 128u * half + 64u * b + lane_off;
+                float sc[kKeys];
+                tc::tmem_ld32(tS, sc);
+                tc::tmem_ld32(tS + 32u, sc + 32);
+                tc::tmem_ld_wait();
+                const int kbase = kv8_chunk(item, item.c0 + t) * kKeys;
+                if (kbase + kKeys - 1 > pos_lo ||
+                    (p.window > 0 && kbase + p.window <= pos_hi && kbase + kKeys > p.sinks)) {
+                    const int low = p.window > 0 ? pos - p.window : -1;
+#pragma unroll
+                    for (int k = 0; k < kKeys; ++k) {
+                        const int key = kbase + k;
+                        if (key > pos || (key <= low && key >= p.sinks)) sc[k] = -INFINITY;
+                    }
+                }
+                // a factor above 0 keeps -inf what it is for rows of zeros
+                const float f = fmaxf(qs * exp2_int(min(max(A - U, -126), 127)), 1.2e-38f);
+                float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+                for (int k = 4; k < kKeys; ++k) mx[k & 3] = fmaxf(mx[k & 3], sc[k]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                const float mn = top > m + kMargin ? top : m;
+                const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+                const float alpha = ex2_ftz(m - mu);
+                m = mn;
+                if (t > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    // O must hold the previous tile's products before it is rescaled
+                    if (!wait_all(&ctl->o_full[half][b ^ 1u], ((hn - 1) >> 1) & 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float ov[32];
+                        tc::tmem_ld32(tO + c * 32u, ov);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) ov[k] *= alpha;
+                        tc::tmem_st32(tO + c * 32u, ov);
+                    }
+                }
+                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t pk[16], rest[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float x = ex2_ftz(fmaf(sc[32 * q + 2 * k], f, -mu));
+                        const float y = ex2_ftz(fmaf(sc[32 * q + 2 * k + 1], f, -mu));
+                        ls[k & 3] += x + y;
+                        pk[k] = pack_bf16(x, y);
+                        if constexpr (NP == 2) rest[k] = pack_rest(x, y, pk[k]);
+                    }
+                    tc::tmem_st16(tS + 16u * q, pk);
+                    if constexpr (NP == 2) tc::tmem_st16(tS + 32u + 16u * q, rest);
+                }
+                l = fmaf(l, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+                tc::tmem_st_wait();
+                tc::fence_before_sync();
+                mbar_arrive(&ctl->p_full[half][b]);
+            }
+            if (ok && half < halves) {
+                const uint32_t hn = hn0 + ntiles - 1;
+                if (wait_all(&ctl->o_full[half][hn & 1u], (hn >> 1) & 1u)) {
+                    tc::fence_after_sync();
+                    const bool whole = item.slot < 0;
+                    const float scale = whole ? 1.0f / l : 1.0f;
+                    const int64_t slot = (int64_t(item.slot) * H + h) * kRows + half * kHalf + r;
+                    T* dst = static_cast<T*>(p.out) + int64_t(q0 + row / p.group) * p.out_stride +
+                             int64_t(h * p.group + row % p.group) * HD;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float ov[32];
+                        tc::tmem_ld32(tO + c * 32u, ov);
+                        tc::tmem_ld_wait();
+                        if (!live) continue;
+                        // columns 4 k + (0, 1, 2, 3) are dims 4 k + (0, 2, 1, 3)
+#pragma unroll
+                        for (int k = 1; k < 32; k += 4) {
+                            const float x = ov[k];
+                            ov[k] = ov[k + 1];
+                            ov[k + 1] = x;
+                        }
+                        if (whole) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint4 raw;
+                                T* v = reinterpret_cast<T*>(&raw);
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) v[q] = from_float<T>(ov[8 * k + q] * scale);
+                                reinterpret_cast<uint4*>(dst + c * 32)[k] = raw;
+                            }
+                        } else {
+                            float4* acc = reinterpret_cast<float4*>(w.acc + slot * HD + c * 32);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                acc[k] = make_float4(ov[4 * k] * scale, ov[4 * k + 1] * scale, ov[4 * k + 2] * scale,
+                                                     ov[4 * k + 3] * scale);
+                            }
+                        }
+                    }
+                    if (live && !whole) w.ml[slot] = make_float2(m, l);
+                }
+            }
+            tc::fence_before_sync();
+            done(job);
+        }
+    } else if (warp < kMmaWarp) {
+        // ------------------------------------------------------------- converters
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+        for (uint32_t j = 0;; ++j) {
+            const int it = next_item(j);
+            if (it < 0) break;
+            const Job job = job_of(it);
+            const Kv8Item& item = job.item;
+            const int h = job.h, ntiles = job.ntiles, pos_lo = job.pos_lo, pos_hi = job.pos_hi;
+            const uint32_t n0 = seq;
+            const int ct = tid - 32 * kConvWarp0;
+            const int piece = ct % S::PIECES;
+            const int row0 = ct / S::PIECES;
+            const int32_t* table = p.block_tables + int64_t(item.seq) * p.max_blocks;
+            const int64_t column = int64_t(h) * HD + piece * 16;
+            // lane l finds positions l and l + 32 of a tile: the table's entry, or
+            // kNone where no row sees, and the slot
+            constexpr int kNone = INT32_MIN;
+            struct Where {
+                int blk[2], in[2];
+            };
+            auto find = [&](int c) -> Where {
+                Where x;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int pos = kv8_chunk(item, c) * kKeys + 32 * i + lane;
+                    x.blk[i] = kNone;
+                    x.in[i] = 0;
+                    if (c < item.c1 && pos <= pos_hi &&
+                        (p.window <= 0 || pos > pos_lo - p.window || pos < p.sinks)) {
+                        const int at = pos / p.a.block_size;
+                        x.in[i] = pos - at * p.a.block_size;
+                        x.blk[i] = table[at];
+                    }
+                }
+                return x;
+            };
+            struct Raw {
+                uint4 k[S::COPIES], v[S::COPIES];
+                int ke[2], ve[2];  // exponents of positions l, l + 32
+            };
+            auto load = [&](Where x, Raw& r) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    r.ke[i] = r.ve[i] = -1000;  // nothing there
+                    if (x.blk[i] != kNone && (x.blk[i] < 0 || x.blk[i] >= p.a.num_blocks)) {
+                        raise_status(kStatusBounds);
+                        x.blk[i] = kNone;
+                    }
+                    if (x.blk[i] >= 0) {
+                        const int64_t at = int64_t(x.blk[i]) * p.a.exp_block_stride +
+                                           int64_t(h) * p.a.block_size + x.in[i];
+                        r.ke[i] = __ldg(p.a.k_exps + at);
+                        r.ve[i] = __ldg(p.a.v_exps + at);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int row = row0 + S::STEP * i;
+                    // rows 0..31 live in element 0; a thread's row i is on one side of 32
+                    const int blk0 = __shfl_sync(0xffffffffu, x.blk[0], row & 31);
+                    const int blk1 = __shfl_sync(0xffffffffu, x.blk[1], row & 31);
+                    const int in0 = __shfl_sync(0xffffffffu, x.in[0], row & 31);
+                    const int in1 = __shfl_sync(0xffffffffu, x.in[1], row & 31);
+                    const int blk = row < 32 ? blk0 : blk1, in = row < 32 ? in0 : in1;
+                    r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);
+                    if (blk >= 0) {
+                        const int64_t at = int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + column;
+                        r.k[i] = __ldg(reinterpret_cast<const uint4*>(p.a.k_codes + at));
+                        r.v[i] = __ldg(reinterpret_cast<const uint4*>(p.a.v_codes + at));
+                    }
+                }
+            };
+            // One tensor into a stage: atom piece / 4, the two 16-byte chunks of the
+            // piece swizzled by the row; pieces of the second atom write theirs in
+            // the other order, so that 8 lanes reach 8 places of the banks.
+            auto put = [&](unsigned char* dst, int row, uint4 a, uint4 b) {
+                unsigned char* at = dst + (piece >> 2) * S::ATOM + row * 128;
+                const int c = (piece & 3) * 2, swap = (piece >> 2) & 1;
+                *reinterpret_cast<uint4*>(at + ((c + swap) ^ (row & 7)) * 16) = swap ? b : a;
+                *reinterpret_cast<uint4*>(at + ((c + 1 - swap) ^ (row & 7)) * 16) = swap ? a : b;
+            };
+            auto exp_of = [&](const int* e, int row) {
+                const int e0 = __shfl_sync(0xffffffffu, e[0], row & 31);
+                const int e1 = __shfl_sync(0xffffffffu, e[1], row & 31);
+                return row < 32 ? e0 : e1;
+            };
+            auto convert_k = [&](unsigned char* dst, const Raw& r, int top) {
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int row = row0 + S::STEP * i;
+                    const __half2 f = half_power(exp_of(r.ke, row) - top + U);
+                    uint4 a, b;
+                    scaled_half4<kFormat>(r.k[i].x, f, a.x, a.y);
+                    scaled_half4<kFormat>(r.k[i].y, f, a.z, a.w);
+                    scaled_half4<kFormat>(r.k[i].z, f, b.x, b.y);
+                    scaled_half4<kFormat>(r.k[i].w, f, b.z, b.w);
+                    put(dst, row, a, b);
+                }
+            };
+            auto convert_v = [&](unsigned char* dst, const Raw& r) {
+                // E4M3 above 2^7 would need a factor beyond bf16's range: the rest of
+                // it is a second factor, which almost no tile has
+                constexpr int kBias = kFormat == NVLLM_KV8_E4M3 ? 120 : 0;
+                const bool large = kBias > 0 && __any_sync(0xffffffffu, max(r.ve[0], r.ve[1]) > 7);
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int row = row0 + S::STEP * i;
+                    const int e = exp_of(r.ve, row);
+                    const __nv_bfloat162 f = __float2bfloat162_rn(exp2_int(min(max(e, -126) + kBias, 127)));
+                    uint32_t o[8];
+                    scaled_bf16x4<kFormat>(r.v[i].x, f, o[0], o[1]);
+                    scaled_bf16x4<kFormat>(r.v[i].y, f, o[2], o[3]);
+                    scaled_bf16x4<kFormat>(r.v[i].z, f, o[4], o[5]);
+                    scaled_bf16x4<kFormat>(r.v[i].w, f, o[6], o[7]);
+                    if (large) {
+                        const __nv_bfloat162 g = __float2bfloat162_rn(exp2_int(max(e - 7, 0)));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const __nv_bfloat162 x = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[k]), g);
+                            o[k] = *reinterpret_cast<const uint32_t*>(&x);
+                        }
+                    }
+                    put(dst, row, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
+                }
+            };
+            Raw raw[2];
+            Where next = find(item.c0);
+            load(next, raw[0]);
+            next = find(item.c0 + 1);
+            bool ok = true;
+            auto step = [&](int t, Raw& now, Raw& then) -> bool {
+                const uint32_t n = n0 + t;
+                const uint32_t st = n % kStages;
+                if (t + 1 < ntiles) {
+                    load(next, then);
+                    next = find(item.c0 + t + 2);
+                }
+                const int A = max(__reduce_max_sync(0xffffffffu, max(now.ke[0], now.ke[1])), kKv8MinExp);
+                if (n >= uint32_t(kStages) && !wait_all(&ctl->st_free[st], (n / kStages - 1) & 1u)) return false;
+                unsigned char* stage = sKV + st * S::STAGE;
+                if (ct == 0) ctl->top[st] = A;
+                convert_k(stage, now, A);
+                tc::fence_async_smem();
+                mbar_arrive(&ctl->kc_full[st]);
+                convert_v(stage + S::TILE, now);
+                tc::fence_async_smem();
+                mbar_arrive(&ctl->vc_full[st]);
+                return true;
+            };
+            for (int t = 0; ok && t < ntiles; t += 2) {
+                ok = step(t, raw[0], raw[1]);
+                if (ok && t + 1 < ntiles) ok = step(t + 1, raw[1], raw[0]);
+            }
+            done(job);
+        }
+    } else {
+        // ------------------------------------------------------------------- MMAs
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+        for (uint32_t j = 0; warp == kMmaWarp; ++j) {
+            const int it = next_item(j);
+            if (it < 0) break;
+            const Job job = job_of(it);
+            const int ntiles = job.ntiles, halves = job.halves;
+            const uint32_t n0 = seq;
+            auto issue_s = [&](uint32_t n) -> bool {
+                if (!wait_all(&ctl->kc_full[n % kStages], (n / kStages) & 1u)) return false;
+                // S goes where P of the key tile two back was: its O must be complete
+                for (int i = 0; i < halves; ++i) {
+                    const uint32_t hn = (i ? seq1 : seq) + (n - n0);
+                    if (n - n0 >= 2 && !wait_all(&ctl->o_full[i][hn & 1u], ((hn - 2) >> 1) & 1u)) return false;
+                }
+                if (lane == 0) {
+                    tc::fence_after_sync();
+                    const uint32_t k0 = smem_addr(sKV + n % kStages * S::STAGE);
+                    for (int i = 0; i < halves; ++i) {
+                        const uint32_t a0 = smem_addr(sQ + i * S::Q_HALF);
+                        const uint32_t hn = (i ? seq1 : seq) + (n - n0);
+                        const uint32_t d = tmem + 128u * i + 64u * (hn & 1u);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint32_t in = (k & 3) * 32u;
+                            tc::mma_f16(d, tc::sw128_desc(a0 + (k >> 2) * S::Q_ATOM + in, 16, 1024),
+                                        tc::sw128_desc(k0 + (k >> 2) * S::ATOM + in, 16, 1024), kIdescS, k > 0);
+                        }
+                        tc::commit(&ctl->s_full[i][hn & 1u]);
+                    }
+                    issued_mma = true;
+                }
+                __syncwarp();
+                return true;
+            };
+            bool ok = wait_all(&ctl->q_full, j & 1u) && issue_s(n0);
+            for (int t = 0; ok && t < ntiles; ++t) {
+                const uint32_t n = n0 + t;
+                if (t + 1 < ntiles && !issue_s(n + 1)) break;
+                ok = wait_all(&ctl->vc_full[n % kStages], (n / kStages) & 1u);
+                for (int i = 0; ok && i < halves; ++i) {
+                    const uint32_t hn = (i ? seq1 : seq) + t;
+                    ok = wait_all(&ctl->p_full[i][hn & 1u], (hn >> 1) & 1u);
+                    if (ok && lane == 0) {
+                        tc::fence_after_sync();
+                        const uint32_t v0 = smem_addr(sKV + n % kStages * S::STAGE + S::TILE);
+                        const uint32_t pb = tmem + 128u * i + 64u * (hn & 1u);
+                        const uint32_t d = tmem + 256u + 128u * i;
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k) {
+                            const uint64_t v = tc::sw128_desc(v0 + k * 2048u, S::ATOM, 1024);
+                            tc::mma_f16_ts(d, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
+                            if constexpr (NP == 2) tc::mma_f16_ts(d, pb + 32u + 8u * k, v, kIdescO, true);
+                        }
+                        tc::commit(&ctl->o_full[i][hn & 1u]);
+                        if (i + 1 == halves) tc::commit(&ctl->st_free[n % kStages]);
+                    }
+                    __syncwarp();
+                }
+            }
+            done(job);
+        }
+    }
+
+    // Teardown: on an abort, let this CTA's MMAs finish (bounded) before its
+    // shared memory and TMEM are released.
+    if (warp == kMmaWarp && lane == 0 && issued_mma) {
+        tc::commit(&ctl->drain);
+        mbar_wait(&ctl->drain, 0, kStatusInKv8Tc);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <typename T, int kFormat, int HD>
+cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
+    auto* k = kv8_attention_tc_kernel<T, kFormat, HD>;
+    static bool ready[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<HD>::SMEM));
+        if (e != cudaSuccess) return e;
+        ready[dev] = true;
+    }
+    return launch_programmatic(k, dim3(kSms), dim3(kThreads), Shape<HD>::SMEM, st, p, w);
+}
+
+template <typename T, int kFormat>
+cudaError_t launch_hd(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t st) {
+    return p.a.head_dim == 64 ? launch_kernel<T, kFormat, 64>(p, w, st) : launch_kernel<T, kFormat, 128>(p, w, st);
+}
+
+template <typename T>
+cudaError_t launch_type(const Kv8AttnParams& p, const Kv8Work& w, int32_t format, cudaStream_t st) {
+    return format == NVLLM_KV8_E4M3 ? launch_hd<T, NVLLM_KV8_E4M3>(p, w, st)
+                                    : launch_hd<T, NVLLM_KV8_INT8>(p, w, st);
+}
+
+}  // namespace
+
+bool kv8_tc_supported(int32_t dtype, int32_t head_dim) {
+    return dtype != NVLLM_DTYPE_FP32 && (head_dim == 64 || head_dim == 128);
+}
+
+Kv8Work kv8_tc_work() {
+    Kv8Work w{};
+    w.tile_rows = kRows;
+    w.chunk = kKeys;
+    w.min_run = 8;
+    w.target = kSms;
+    return w;
+}
+
+cudaError_t launch_kv8_tc(const Kv8AttnParams& p, const Kv8Work& w, int32_t dtype, int32_t format,
+                          cudaStream_t stream) {
+    return dtype == NVLLM_DTYPE_BF16 ? launch_type<__nv_bfloat16>(p, w, format, stream)
+                                     : launch_type<__half>(p, w, format, stream);
+}
+
+}  // namespace nvllm

@@ -66,6 +66,7 @@ class Sizes(NamedTuple):
     wide: np.ndarray  # max_j scale max_d|q_d| sum_d |K_jd|
     top: np.ndarray   # max_j w_j max_d|V_jd|
     n: np.ndarray     # visible positions
+    far: np.ndarray   # scale sum_d|q_d| max|K| over all positions, seen or not
 
 
 def attention(q, k, v, first_pos: int, group: int, scale: float, window: int = 0, sinks: int = 0):
@@ -88,7 +89,8 @@ def attention(q, k, v, first_pos: int, group: int, scale: float, window: int = 0
     wide = np.where(seen[:, None], np.abs(kk).sum(-1).T[None], 0.0).max(-1) * np.abs(q).max(-1) * scale
     top = (w * np.abs(vv).max(-1).T[None]).max(-1)
     n = np.broadcast_to(seen.sum(-1)[:, None], (rows, H))
-    return np.einsum("rhj,jhd->rhd", w, vv), Sizes(np.einsum("rhj,jhd->rhd", w, np.abs(vv)), mag, wide, top, n)
+    return np.einsum("rhj,jhd->rhd", w, vv), Sizes(np.einsum("rhj,jhd->rhd", w, np.abs(vv)), mag, wide, top, n,
+                                                   np.abs(q).sum(-1) * np.abs(kk).max((0, 2)) * scale)
 
 
 # Roundings, relative to the value: half a step of each type.
@@ -110,13 +112,16 @@ def tolerance(out, b: Sizes, hd: int, dtype: str) -> np.ndarray:
     for the scale, the logarithm's base and the exponent's argument). q enters as
     fp16 terms of the row scaled to [1, 2): two leave at most 2^-23 of the row's
     largest element, one (bf16 and fp16 rows) 2^-25 where an element is below
-    2^-14 of it: 2^-23 wide. The exponential adds 2^-22. A weight then is off by
+    2^-14 of it: 2^-23 wide. In the kernel for many rows a key's values are fp16
+    relative to the largest exponent A of 64 keys, in steps of 2^(A - 30) at the
+    coarsest (INT8; 2^(A - 32) for E4M3), where the largest key reaches 2^(A + 6)
+    (2^(A + 7)): 2^-36 far. The exponential adds 2^-22. A weight then is off by
     exp(ds) - 1, the sum of the weights by as much plus its n additions, and the
     sum with V by n additions more. A weight is rounded relative to itself, but to
     no less than 2^-25 of the largest contribution w_j 2^(e_j) (an fp16 step
     below 2^-14); times a code that is at most M 2^(e_j) < 2 max_d|V_jd|: n
     2^-24 top in all. The output's own rounding comes on top."""
-    ds = (hd + 8) * 2.0 ** -23 * b.mag + 2.0 ** -23 * b.wide + 2.0 ** -22
+    ds = (hd + 8) * 2.0 ** -23 * b.mag + 2.0 ** -23 * b.wide + 2.0 ** -36 * b.far + 2.0 ** -22
     rel = 2 * np.expm1(ds) + (2 * b.n + 16) * 2.0 ** -23 + WEIGHT[dtype]
     return (rel[..., None] * b.vabs + (b.n * b.top)[..., None] * 2.0 ** -24 + HALF[dtype] * np.abs(out)
             + SMALLEST[dtype])
