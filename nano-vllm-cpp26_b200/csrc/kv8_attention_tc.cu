@@ -656,36 +656,44 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     } else {
         // ------------------------------------------------------------------- MMAs
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+        // operand descriptors, built once: offsets are added to their address field
+        // (16-byte units), since one thread's instructions pace the MMAs
+        // what they are built from is made warp-uniform, so that it lives in uniform
+        // registers, where the instructions take it from
+        auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+        const uint32_t utmem = uniform(tmem);
+        const uint64_t q_desc = tc::sw128_desc(uniform(smem_addr(sQ)), 16, 1024);
+        const uint64_t k_desc = tc::sw128_desc(uniform(smem_addr(sKV)), 16, 1024);
+        const uint64_t v_desc = tc::sw128_desc(uniform(smem_addr(sKV + S::TILE)), S::ATOM, 1024);
         for (uint32_t j = 0; warp == kMmaWarp; ++j) {
             const int it = next_item(j);
             if (it < 0) break;
             const Job job = job_of(it);
-            const int ntiles = job.ntiles, halves = job.halves;
-            const uint32_t n0 = seq;
+            const int ntiles = int(uniform(uint32_t(job.ntiles))), halves = int(uniform(uint32_t(job.halves)));
+            const uint32_t n0 = uniform(seq), h1 = uniform(seq1);
             auto issue_s = [&](uint32_t n) -> bool {
                 if (!wait_all(&ctl->kc_full[n % kStages], (n / kStages) & 1u)) return false;
                 // S goes where P of the key tile two back was: its O must be complete
                 for (int i = 0; i < halves; ++i) {
-                    const uint32_t hn = (i ? seq1 : seq) + (n - n0);
+                    const uint32_t hn = (i ? h1 : n0) + (n - n0);
                     if (n - n0 >= 2 && !wait_all(&ctl->o_full[i][hn & 1u], ((hn - 2) >> 1) & 1u)) return false;
                 }
-                if (lane == 0) {
+                if (tc::elect_one()) {
                     tc::fence_after_sync();
-                    const uint32_t k0 = smem_addr(sKV + n % kStages * S::STAGE);
+                    const uint64_t kd = k_desc + n % kStages * (S::STAGE >> 4);
                     for (int i = 0; i < halves; ++i) {
-                        const uint32_t a0 = smem_addr(sQ + i * S::Q_HALF);
-                        const uint32_t hn = (i ? seq1 : seq) + (n - n0);
-                        const uint32_t d = tmem + 128u * i + 64u * (hn & 1u);
+                        const uint32_t hn = (i ? h1 : n0) + (n - n0);
+                        const uint32_t d = utmem + 128u * i + 64u * (hn & 1u);
+                        const uint64_t qd = q_desc + i * (S::Q_HALF >> 4);
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k) {
-                            const uint32_t in = (k & 3) * 32u;
-                            tc::mma_f16(d, tc::sw128_desc(a0 + (k >> 2) * S::Q_ATOM + in, 16, 1024),
-                                        tc::sw128_desc(k0 + (k >> 2) * S::ATOM + in, 16, 1024), kIdescS, k > 0);
+                            tc::mma_f16(d, qd + ((k >> 2) * (S::Q_ATOM >> 4) + (k & 3) * 2),
+                                        kd + ((k >> 2) * (S::ATOM >> 4) + (k & 3) * 2), kIdescS, k > 0);
                         }
                         tc::commit(&ctl->s_full[i][hn & 1u]);
                     }
-                    issued_mma = true;
                 }
+                issued_mma = true;
                 __syncwarp();
                 return true;
             };
@@ -695,16 +703,16 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 if (t + 1 < ntiles && !issue_s(n + 1)) break;
                 ok = wait_all(&ctl->vc_full[n % kStages], (n / kStages) & 1u);
                 for (int i = 0; ok && i < halves; ++i) {
-                    const uint32_t hn = (i ? seq1 : seq) + t;
+                    const uint32_t hn = (i ? h1 : n0) + t;
                     ok = wait_all(&ctl->p_full[i][hn & 1u], (hn >> 1) & 1u);
-                    if (ok && lane == 0) {
+                    if (ok && tc::elect_one()) {
                         tc::fence_after_sync();
-                        const uint32_t v0 = smem_addr(sKV + n % kStages * S::STAGE + S::TILE);
-                        const uint32_t pb = tmem + 128u * i + 64u * (hn & 1u);
-                        const uint32_t d = tmem + 256u + 128u * i;
+                        const uint64_t vd = v_desc + n % kStages * (S::STAGE >> 4);
+                        const uint32_t pb = utmem + 128u * i + 64u * (hn & 1u);
+                        const uint32_t d = utmem + 256u + 128u * i;
 #pragma unroll
                         for (int k = 0; k < kKeys / 16; ++k) {
-                            const uint64_t v = tc::sw128_desc(v0 + k * 2048u, S::ATOM, 1024);
+                            const uint64_t v = vd + k * (2048 >> 4);
                             tc::mma_f16_ts(d, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
                             if constexpr (NP == 2) tc::mma_f16_ts(d, pb + 32u + 8u * k, v, kIdescO, true);
                         }
@@ -720,7 +728,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
     // Teardown: on an abort, let this CTA's MMAs finish (bounded) before its
     // shared memory and TMEM are released.
-    if (warp == kMmaWarp && lane == 0 && issued_mma) {
+    if (warp == kMmaWarp && issued_mma && tc::elect_one()) {
         tc::commit(&ctl->drain);
         mbar_wait(&ctl->drain, 0, kStatusInKv8Tc);
     }

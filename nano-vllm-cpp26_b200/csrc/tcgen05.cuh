@@ -39,6 +39,17 @@ __device__ __forceinline__ void fence_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok));
+    return ok != 0;
+}
+
 // ---- descriptors ------------------------------------------------------------
 // Shared-memory matrix descriptor for a 128-byte-swizzled operand (the layout
 // TMA writes with CU_TENSOR_MAP_SWIZZLE_128B): start address, leading and
