@@ -29,6 +29,7 @@ struct Kv8Arena {
     int64_t exp_block_stride;  // exponents from block to block
     int64_t num_blocks;
     int32_t block_size;
+    int32_t block_shift;  // log2 of block_size where it is a power of two, else -1
     int32_t num_heads;  // KV heads
     int32_t head_dim;
 };
@@ -116,6 +117,22 @@ size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_
 cudaError_t launch_kv8_plan(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t stream);
 cudaError_t launch_kv8_merge(const Kv8AttnParams& p, const Kv8Work& w, int32_t dtype,
                              cudaStream_t stream);
+
+// Block-table entry and slot of a position.
+__device__ __forceinline__ void kv8_place(const Kv8Arena& a, int pos, int& entry, int& slot) {
+    entry = a.block_shift >= 0 ? pos >> a.block_shift : pos / a.block_size;
+    slot = pos - entry * a.block_size;
+}
+
+// 16 bytes from global to shared memory, or zeros where there is nothing to read.
+__device__ __forceinline__ void kv8_copy16(uint32_t dst, const unsigned char* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void kv8_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void kv8_copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // Position of entry c of a tile's list, in chunks.
 __device__ __forceinline__ int kv8_chunk(const Kv8Item& it, int c) {

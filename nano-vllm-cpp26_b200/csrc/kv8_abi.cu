@@ -39,6 +39,10 @@ int prepare_arena(Kv8Arena& a, const nvllm_kv8_arena* arena, int32_t layer,
     a.exp_block_stride = g.num_layers * exp_layer;
     a.num_blocks = g.num_blocks;
     a.block_size = g.block_size;
+    a.block_shift = -1;
+    for (int i = 0; i < 31; ++i) {
+        if (g.block_size == (1 << i)) a.block_shift = i;
+    }
     a.num_heads = g.num_heads;
     a.head_dim = g.head_dim;
     return NVLLM_OK;

@@ -83,16 +83,6 @@ __device__ __forceinline__ Piece<BYTES> read_piece(const unsigned char* p) {
     return r;
 }
 
-// 16 bytes, or zeros where there is nothing to read.
-__device__ __forceinline__ void copy16(uint32_t dst, const unsigned char* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Four codes -> two pairs of fp16, in order.
 template <int kFormat>
 __device__ __forceinline__ void to_half4(uint32_t w, uint32_t& a, uint32_t& b) {
@@ -365,8 +355,10 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
         auto seen = [&](int j) {
             return j <= pos_hi && (p.window <= 0 || j > pos_lo - p.window || j < p.sinks);
         };
-        auto block_at = [&](int j) -> int {
-            const int b = table[j / p.a.block_size];
+        auto block_at = [&](int j, int& slot) -> int {
+            int entry;
+            kv8_place(p.a, j, entry, slot);
+            const int b = table[entry];
             if (b >= 0 && b < p.a.num_blocks) return b;
             raise_status(kStatusBounds);
             return -1;
@@ -389,8 +381,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     if (cc < item.c1) {
                         const int j = base_of(cc) + lane % SUB * kSub;
                         if (j <= pos_hi && (p.window <= 0 || j + kSub - 1 > pos_lo - p.window || j < p.sinks)) {
-                            ahead_blk = block_at(j);
-                            ahead_in = j % p.a.block_size;
+                            ahead_blk = block_at(j, ahead_in);
                         }
                     }
                 }
@@ -398,8 +389,8 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 x.in = __shfl_sync(0xffffffffu, ahead_in, at & 31);
             } else {
                 const int j = base_of(c) + u * kSub + (lane & 15);
-                x.blk = seen(j) ? block_at(j) : -1;
-                x.in = j % p.a.block_size;
+                x.in = 0;
+                x.blk = seen(j) ? block_at(j, x.in) : -1;
             }
             x.exps = 0;
             if (x.blk >= 0) {
@@ -435,8 +426,8 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     const bool on = blk >= 0 && (!kB16 || all || seen(base + u * kSub + row));
                     const int64_t at = on ? int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + piece : 0;
                     const uint32_t to = dst + R::at(row, lane % R::PIECES * 16);
-                    copy16(to, p.a.k_codes + at, on);
-                    copy16(to + R::TILE, p.a.v_codes + at, on);
+                    kv8_copy16(to, p.a.k_codes + at, on);
+                    kv8_copy16(to + R::TILE, p.a.v_codes + at, on);
                 }
             }
             return r;
@@ -452,9 +443,9 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             const int c = item.c0 + warp;
             Exps first{};
             if (c < item.c1) first = issue(c, 0, 0);
-            copy_commit();
+            kv8_copy_commit();
             if (c + kWarps < item.c1) ahead = issue(c + kWarps, 1, 1);
-            copy_commit();
+            kv8_copy_commit();
             store_exps(first, 0);
         }
 
@@ -527,7 +518,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
         for (int c = item.c0 + warp, n = 0; c < item.c1; c += kWarps, ++n) {
             const int buf = n & 1;
-            copy_wait<1>();
+            kv8_copy_wait<1>();
             store_exps(ahead, buf ^ 1);
             __syncwarp();
             const unsigned char* sK = ring + buf * S::BUF;
@@ -702,11 +693,11 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             }
             __syncwarp();  // the buffer is free
             if (c + 2 * kWarps < item.c1) ahead = issue(c + 2 * kWarps, n + 2, buf);
-            copy_commit();
+            kv8_copy_commit();
         }
 
         // ---- join the warps ---------------------------------------------------------
-        copy_wait<0>();
+        kv8_copy_wait<0>();
         __syncthreads();  // the buffers are read no more
         // Lane (g, t) holds dims VB g + 8 VB q + 2 k + e (tile (q, k), half e) of its rows
 #pragma unroll

@@ -26,10 +26,11 @@
 //                   softmax works on S(n), then O(n) += P(n) V(n) of each half.
 //                   Its warpgroup (three more warps that do nothing) gives its
 //                   registers to the softmax.
-//   warps 8-11      converters: 16 codes per thread from the arenas to registers a
-//                   tile ahead (block ids two ahead), then as fp16 into a ring of
-//                   three stages in the MMA's 128-byte swizzle; rows that no query
-//                   of the tile sees become zeros.
+//   warps 8-11      converters: 16-byte pieces of codes by asynchronous copies two
+//                   key tiles ahead (block ids three ahead) into a place of the
+//                   thread's own, so that no one else waits for them, then as
+//                   16-bit floats into a ring of three stages in the MMA's
+//                   128-byte swizzle; rows that no query of the tile sees are 0.
 // TMEM (512 columns): S of half i, buffer b at 128 i + 64 b, O of half i at 256 +
 // 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
 // special function units, as many as the products take on the tensor cores at
@@ -50,6 +51,7 @@ constexpr int kHalf = 128;           // rows of a half (TMEM lanes)
 constexpr int kRows = 2 * kHalf;     // rows of a tile
 constexpr int kKeys = 64;            // keys of a key tile
 constexpr int kStages = 3;
+constexpr int kRaw = 3;              // key tiles of codes on their way or landed
 constexpr int kConvWarp0 = 8;
 constexpr int kConvThreads = 128;
 constexpr int kMmaWarp = 12;
@@ -105,7 +107,9 @@ struct Shape {
     static constexpr uint32_t Q_HALF = Q_ATOM * (HD / 64);
     static constexpr uint32_t OFF_Q = 0;
     static constexpr uint32_t OFF_KV = 2 * Q_HALF;
-    static constexpr uint32_t OFF_CTL = OFF_KV + kStages * STAGE;
+    static constexpr uint32_t RAW = 2 * kKeys * HD;         // codes of a key tile
+    static constexpr uint32_t OFF_RAW = OFF_KV + kStages * STAGE;
+    static constexpr uint32_t OFF_CTL = OFF_RAW + kRaw * RAW;
     static constexpr uint32_t SMEM = OFF_CTL + 512 + 1024;  // + control block + alignment slack
     static_assert(SMEM <= 227u * 1024u, "shared memory");
     static_assert(sizeof(Control) <= 512, "control block");
@@ -133,6 +137,33 @@ __device__ __forceinline__ float ex2_ftz(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two floats by one instruction, and the largest of three.
+__device__ __forceinline__ uint64_t pair(float2 a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
@@ -408,8 +439,13 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const float f = fmaxf(qs * exp2_int(min(max(A - U, -126), 127)), 1.2e-38f);
                 float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-                for (int k = 4; k < kKeys; ++k) mx[k & 3] = fmaxf(mx[k & 3], sc[k]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                for (int k = 4; k < kKeys; k += 8) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        mx[q] = k + 4 + q < kKeys ? max3(mx[q], sc[k + q], sc[k + 4 + q]) : fmaxf(mx[q], sc[k + q]);
+                    }
+                }
+                const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * f;
                 const float mn = top > m + kMargin ? top : m;
                 const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
                 const float alpha = ex2_ftz(m - mu);
@@ -431,22 +467,23 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                         tc::tmem_st32(tO + c * 32u, ov);
                     }
                 }
-                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+                float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 f2 = make_float2(f, f), mu2 = make_float2(-mu, -mu);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     uint32_t pk[16], rest[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float x = ex2_ftz(fmaf(sc[32 * q + 2 * k], f, -mu));
-                        const float y = ex2_ftz(fmaf(sc[32 * q + 2 * k + 1], f, -mu));
-                        ls[k & 3] += x + y;
-                        pk[k] = pack_bf16(x, y);
-                        if constexpr (NP == 2) rest[k] = pack_rest(x, y, pk[k]);
+                        float2 x = fma2(make_float2(sc[32 * q + 2 * k], sc[32 * q + 2 * k + 1]), f2, mu2);
+                        x = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
+                        ls[k & 1] = add2(ls[k & 1], x);
+                        pk[k] = pack_bf16(x.x, x.y);
+                        if constexpr (NP == 2) rest[k] = pack_rest(x.x, x.y, pk[k]);
                     }
                     tc::tmem_st16(tS + 16u * q, pk);
                     if constexpr (NP == 2) tc::tmem_st16(tS + 32u + 16u * q, rest);
                 }
-                l = fmaf(l, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+                l = fmaf(l, alpha, (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
                 mbar_arrive(&ctl->p_full[half][b]);
@@ -500,6 +537,20 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     } else if (warp < kMmaWarp) {
         // ------------------------------------------------------------- converters
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+        const int ct = tid - 32 * kConvWarp0;
+        const int piece = ct % S::PIECES;
+        const int row0 = ct / S::PIECES;
+        unsigned char* sRaw = base + S::OFF_RAW;
+        const uint32_t raw_addr = smem_addr(sRaw) + ct * 16;
+        uint32_t raw_slot = 0;  // of the next tile to convert
+        // Where the thread's piece goes: atom piece / 4, two 16-byte chunks swizzled by
+        // the row (STEP is a multiple of 8: the same for all its rows). Pieces of the
+        // second atom write theirs in the other order, so that the 8 lanes of a row
+        // reach 8 places of the banks.
+        const int swap = (piece >> 2) & 1;
+        const uint32_t put_row = (piece >> 2) * S::ATOM + row0 * 128;
+        const uint32_t put0 = put_row + (((piece & 3) * 2 + swap) ^ (row0 & 7)) * 16;
+        const uint32_t put1 = put_row + (((piece & 3) * 2 + 1 - swap) ^ (row0 & 7)) * 16;
         for (uint32_t j = 0;; ++j) {
             const int it = next_item(j);
             if (it < 0) break;
@@ -507,152 +558,161 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
             const Kv8Item& item = job.item;
             const int h = job.h, ntiles = job.ntiles, pos_lo = job.pos_lo, pos_hi = job.pos_hi;
             const uint32_t n0 = seq;
-            const int ct = tid - 32 * kConvWarp0;
-            const int piece = ct % S::PIECES;
-            const int row0 = ct / S::PIECES;
             const int32_t* table = p.block_tables + int64_t(item.seq) * p.max_blocks;
             const int64_t column = int64_t(h) * HD + piece * 16;
-            // lane l finds positions l and l + 32 of a tile: the table's entry, or
-            // kNone where no row sees, and the slot
+            const int64_t exp_head = int64_t(h) * p.a.block_size;
+            // lane l finds positions l and l + 32 of a tile: the table's entry (kNone
+            // where no row sees) and the slot
             constexpr int kNone = INT32_MIN;
             struct Where {
                 int blk[2], in[2];
             };
             auto find = [&](int c) -> Where {
                 Where x;
+                const int kbase = kv8_chunk(item, c) * kKeys + lane;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int pos = kv8_chunk(item, c) * kKeys + 32 * i + lane;
+                    const int pos = kbase + 32 * i;
                     x.blk[i] = kNone;
                     x.in[i] = 0;
                     if (c < item.c1 && pos <= pos_hi &&
                         (p.window <= 0 || pos > pos_lo - p.window || pos < p.sinks)) {
-                        const int at = pos / p.a.block_size;
-                        x.in[i] = pos - at * p.a.block_size;
-                        x.blk[i] = table[at];
+                        int entry;
+                        kv8_place(p.a, pos, entry, x.in[i]);
+                        x.blk[i] = __ldg(table + entry);
                     }
                 }
                 return x;
             };
-            struct Raw {
-                uint4 k[S::COPIES], v[S::COPIES];
-                int ke[2], ve[2];  // exponents of positions l, l + 32
-            };
-            auto load = [&](Where x, Raw& r) {
+            auto check = [&](Where& x) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    r.ke[i] = r.ve[i] = -1000;  // nothing there
                     if (x.blk[i] != kNone && (x.blk[i] < 0 || x.blk[i] >= p.a.num_blocks)) {
                         raise_status(kStatusBounds);
                         x.blk[i] = kNone;
                     }
+                }
+            };
+            struct Exps {
+                int k[2], v[2];  // of positions l, l + 32
+            };
+            auto load_exps = [&](const Where& x) -> Exps {
+                Exps e;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    e.k[i] = e.v[i] = -1000;  // nothing there
                     if (x.blk[i] >= 0) {
-                        const int64_t at = int64_t(x.blk[i]) * p.a.exp_block_stride +
-                                           int64_t(h) * p.a.block_size + x.in[i];
-                        r.ke[i] = __ldg(p.a.k_exps + at);
-                        r.ve[i] = __ldg(p.a.v_exps + at);
+                        const int64_t at = int64_t(x.blk[i]) * p.a.exp_block_stride + exp_head + x.in[i];
+                        e.k[i] = __ldg(p.a.k_exps + at);
+                        e.v[i] = __ldg(p.a.v_exps + at);
                     }
                 }
+                return e;
+            };
+            // the thread's rows of a tile are row0 + STEP i; row r's finder is lane
+            // r % 32, element r / 32, which depends on i alone
+            auto copy = [&](const Where& x, uint32_t slot) {
+                const uint32_t dst = raw_addr + slot * S::RAW;
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
-                    const int row = row0 + S::STEP * i;
-                    // rows 0..31 live in element 0; a thread's row i is on one side of 32
-                    const int blk0 = __shfl_sync(0xffffffffu, x.blk[0], row & 31);
-                    const int blk1 = __shfl_sync(0xffffffffu, x.blk[1], row & 31);
-                    const int in0 = __shfl_sync(0xffffffffu, x.in[0], row & 31);
-                    const int in1 = __shfl_sync(0xffffffffu, x.in[1], row & 31);
-                    const int blk = row < 32 ? blk0 : blk1, in = row < 32 ? in0 : in1;
-                    r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);
-                    if (blk >= 0) {
-                        const int64_t at = int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + column;
-                        r.k[i] = __ldg(reinterpret_cast<const uint4*>(p.a.k_codes + at));
-                        r.v[i] = __ldg(reinterpret_cast<const uint4*>(p.a.v_codes + at));
-                    }
+                    constexpr int kHalfRows = 32;
+                    const int el = S::STEP * i / kHalfRows;
+                    const int from = (row0 + S::STEP * i) & 31;
+                    const int blk = __shfl_sync(0xffffffffu, x.blk[el], from);
+                    const int in = __shfl_sync(0xffffffffu, x.in[el], from);
+                    const int64_t at = int64_t(max(blk, 0)) * p.a.block_stride + int64_t(in) * p.a.row + column;
+                    kv8_copy16(dst + i * 2 * kConvThreads * 16, p.a.k_codes + at, blk >= 0);
+                    kv8_copy16(dst + (2 * i + 1) * kConvThreads * 16, p.a.v_codes + at, blk >= 0);
                 }
             };
-            // One tensor into a stage: atom piece / 4, the two 16-byte chunks of the
-            // piece swizzled by the row; pieces of the second atom write theirs in
-            // the other order, so that 8 lanes reach 8 places of the banks.
-            auto put = [&](unsigned char* dst, int row, uint4 a, uint4 b) {
-                unsigned char* at = dst + (piece >> 2) * S::ATOM + row * 128;
-                const int c = (piece & 3) * 2, swap = (piece >> 2) & 1;
-                *reinterpret_cast<uint4*>(at + ((c + swap) ^ (row & 7)) * 16) = swap ? b : a;
-                *reinterpret_cast<uint4*>(at + ((c + 1 - swap) ^ (row & 7)) * 16) = swap ? a : b;
-            };
-            auto exp_of = [&](const int* e, int row) {
-                const int e0 = __shfl_sync(0xffffffffu, e[0], row & 31);
-                const int e1 = __shfl_sync(0xffffffffu, e[1], row & 31);
-                return row < 32 ? e0 : e1;
-            };
-            auto convert_k = [&](unsigned char* dst, const Raw& r, int top) {
-#pragma unroll
-                for (int i = 0; i < S::COPIES; ++i) {
-                    const int row = row0 + S::STEP * i;
-                    const __half2 f = half_power(exp_of(r.ke, row) - top + U);
-                    uint4 a, b;
-                    scaled_half4<kFormat>(r.k[i].x, f, a.x, a.y);
-                    scaled_half4<kFormat>(r.k[i].y, f, a.z, a.w);
-                    scaled_half4<kFormat>(r.k[i].z, f, b.x, b.y);
-                    scaled_half4<kFormat>(r.k[i].w, f, b.z, b.w);
-                    put(dst, row, a, b);
-                }
-            };
-            auto convert_v = [&](unsigned char* dst, const Raw& r) {
-                // E4M3 above 2^7 would need a factor beyond bf16's range: the rest of
-                // it is a second factor, which almost no tile has
-                constexpr int kBias = kFormat == NVLLM_KV8_E4M3 ? 120 : 0;
-                const bool large = kBias > 0 && __any_sync(0xffffffffu, max(r.ve[0], r.ve[1]) > 7);
-#pragma unroll
-                for (int i = 0; i < S::COPIES; ++i) {
-                    const int row = row0 + S::STEP * i;
-                    const int e = exp_of(r.ve, row);
-                    const __nv_bfloat162 f = __float2bfloat162_rn(exp2_int(min(max(e, -126) + kBias, 127)));
-                    uint32_t o[8];
-                    scaled_bf16x4<kFormat>(r.v[i].x, f, o[0], o[1]);
-                    scaled_bf16x4<kFormat>(r.v[i].y, f, o[2], o[3]);
-                    scaled_bf16x4<kFormat>(r.v[i].z, f, o[4], o[5]);
-                    scaled_bf16x4<kFormat>(r.v[i].w, f, o[6], o[7]);
-                    if (large) {
-                        const __nv_bfloat162 g = __float2bfloat162_rn(exp2_int(max(e - 7, 0)));
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const __nv_bfloat162 x = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[k]), g);
-                            o[k] = *reinterpret_cast<const uint32_t*>(&x);
-                        }
-                    }
-                    put(dst, row, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
-                }
-            };
-            Raw raw[2];
-            Where next = find(item.c0);
-            load(next, raw[0]);
-            next = find(item.c0 + 1);
-            bool ok = true;
-            auto step = [&](int t, Raw& now, Raw& then) -> bool {
+            // copies two tiles ahead, exponents one, block ids three
+            Where w1 = find(item.c0), w2 = find(item.c0 + 1), w3 = find(item.c0 + 2);
+            check(w1);
+            copy(w1, raw_slot);
+            kv8_copy_commit();
+            Exps e1 = load_exps(w1);
+            check(w2);
+            if (ntiles > 1) copy(w2, raw_slot + 1 < kRaw ? raw_slot + 1 : raw_slot + 1 - kRaw);
+            kv8_copy_commit();
+            w1 = w2;
+            for (int t = 0; t < ntiles; ++t) {
                 const uint32_t n = n0 + t;
                 const uint32_t st = n % kStages;
-                if (t + 1 < ntiles) {
-                    load(next, then);
-                    next = find(item.c0 + t + 2);
+                check(w3);
+                if (t + 2 < ntiles) copy(w3, raw_slot + 2 < kRaw ? raw_slot + 2 : raw_slot + 2 - kRaw);
+                kv8_copy_commit();
+                const Exps e = e1;
+                e1 = load_exps(w1);
+                w1 = w3;
+                w3 = find(item.c0 + t + 3);
+                const int A = max(__reduce_max_sync(0xffffffffu, max(e.k[0], e.k[1])), kKv8MinExp);
+                // the factors of the lane's two positions, as pairs
+                constexpr int kBias = kFormat == NVLLM_KV8_E4M3 ? 120 : 0;
+                uint32_t fk[2], fv[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const __half2 a = half_power(e.k[i] - A + U);
+                    const __nv_bfloat162 b =
+                        __float2bfloat162_rn(exp2_int(min(max(e.v[i], -126) + kBias, 127)));
+                    fk[i] = *reinterpret_cast<const uint32_t*>(&a);
+                    fv[i] = *reinterpret_cast<const uint32_t*>(&b);
                 }
-                const int A = max(__reduce_max_sync(0xffffffffu, max(now.ke[0], now.ke[1])), kKv8MinExp);
-                if (n >= uint32_t(kStages) && !wait_all(&ctl->st_free[st], (n / kStages - 1) & 1u)) return false;
+                // E4M3 above 2^7 would need a factor beyond bf16's range: the rest of
+                // it is a second factor, which almost no tile has
+                const bool large = kBias > 0 && __any_sync(0xffffffffu, max(e.v[0], e.v[1]) > 7);
+                if (n >= uint32_t(kStages) && !wait_all(&ctl->st_free[st], (n / kStages - 1) & 1u)) break;
+                kv8_copy_wait<2>();  // this tile's pieces, which this thread copied
+                const unsigned char* raw = sRaw + raw_slot * S::RAW + ct * 16;
                 unsigned char* stage = sKV + st * S::STAGE;
                 if (ct == 0) ctl->top[st] = A;
-                convert_k(stage, now, A);
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int el = S::STEP * i / 32;
+                    const uint32_t f = __shfl_sync(0xffffffffu, fk[el], (row0 + S::STEP * i) & 31);
+                    const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+                    const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 2 * kConvThreads * 16);
+                    uint4 a, b;
+                    scaled_half4<kFormat>(x.x, f2, a.x, a.y);
+                    scaled_half4<kFormat>(x.y, f2, a.z, a.w);
+                    scaled_half4<kFormat>(x.z, f2, b.x, b.y);
+                    scaled_half4<kFormat>(x.w, f2, b.z, b.w);
+                    *reinterpret_cast<uint4*>(stage + put0 + i * S::STEP * 128) = swap ? b : a;
+                    *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
+                }
                 tc::fence_async_smem();
                 mbar_arrive(&ctl->kc_full[st]);
-                convert_v(stage + S::TILE, now);
+                stage += S::TILE;
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int el = S::STEP * i / 32;
+                    const uint32_t f = __shfl_sync(0xffffffffu, fv[el], (row0 + S::STEP * i) & 31);
+                    const __nv_bfloat162 f2 = *reinterpret_cast<const __nv_bfloat162*>(&f);
+                    const uint4 x = *reinterpret_cast<const uint4*>(raw + (2 * i + 1) * kConvThreads * 16);
+                    uint32_t o[8];
+                    scaled_bf16x4<kFormat>(x.x, f2, o[0], o[1]);
+                    scaled_bf16x4<kFormat>(x.y, f2, o[2], o[3]);
+                    scaled_bf16x4<kFormat>(x.z, f2, o[4], o[5]);
+                    scaled_bf16x4<kFormat>(x.w, f2, o[6], o[7]);
+                    if (large) {
+                        const int ev = __shfl_sync(0xffffffffu, e.v[el], (row0 + S::STEP * i) & 31);
+                        const __nv_bfloat162 g = __float2bfloat162_rn(exp2_int(max(ev - 7, 0)));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[k]), g);
+                            o[k] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                    }
+                    const uint4 a = make_uint4(o[0], o[1], o[2], o[3]), b = make_uint4(o[4], o[5], o[6], o[7]);
+                    *reinterpret_cast<uint4*>(stage + put0 + i * S::STEP * 128) = swap ? b : a;
+                    *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
+                }
                 tc::fence_async_smem();
                 mbar_arrive(&ctl->vc_full[st]);
-                return true;
-            };
-            for (int t = 0; ok && t < ntiles; t += 2) {
-                ok = step(t, raw[0], raw[1]);
-                if (ok && t + 1 < ntiles) ok = step(t + 1, raw[1], raw[0]);
+                raw_slot = raw_slot + 1 < kRaw ? raw_slot + 1 : 0;
             }
             done(job);
         }
+        kv8_copy_wait<0>();
     } else {
         // ------------------------------------------------------------------- MMAs
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
