@@ -22,10 +22,10 @@
 //                   a row and its TMEM lane. Reads S, masks ragged tiles, P goes
 //                   back over S as the next product's A operand; O is rescaled
 //                   only when m moves by more than kMargin (rarely).
-//   warp 12         MMAs, one lane: S(n+1) of both halves is queued while the
-//                   softmax works on S(n), then O(n) += P(n) V(n) of each half.
-//                   Its warpgroup (three more warps that do nothing) gives its
-//                   registers to the softmax.
+//   warps 12, 13    MMAs of the first and second half, one lane each: O(n) += P(n)
+//                   V(n), then S(n+2) in P's place, while the softmax works on
+//                   S(n+1). Their warpgroup (two more warps do nothing) gives its
+//                   registers to the others.
 //   warps 8-11      converters: 16-byte pieces of codes by asynchronous copies two
 //                   key tiles ahead (block ids three ahead) into a place of the
 //                   thread's own, so that no one else waits for them, then as
@@ -51,12 +51,13 @@ constexpr int kHalf = 128;           // rows of a half (TMEM lanes)
 constexpr int kRows = 2 * kHalf;     // rows of a tile
 constexpr int kKeys = 64;            // keys of a key tile
 constexpr int kStages = 3;
+constexpr int kTops = 8;             // more than the converters can be ahead of the softmax
 constexpr int kRaw = 3;              // key tiles of codes on their way or landed
 constexpr int kConvWarp0 = 8;
 constexpr int kConvThreads = 128;
 constexpr int kMmaWarp = 12;
 constexpr int kThreads = 512;
-constexpr int kItemReaders = kMmaWarp;  // every working warp but the first converter
+constexpr int kItemReaders = kMmaWarp + 1;  // every working warp but the first converter
 // Registers a thread: 128 at launch (65536 / 512). The MMA's warpgroup falls to 40,
 // which frees 88 x 128; the two softmax warpgroups rise to 160 and the converters
 // to 152, which takes (32 + 32 + 24) x 128.
@@ -82,17 +83,19 @@ constexpr uint32_t idesc(int M, int N, bool bf16, bool b_mn) {
 }
 
 struct Control {
-    uint64_t kc_full[kStages];  // K' of a stage written (every converter thread)
-    uint64_t vc_full[kStages];  // V' of a stage written
-    uint64_t st_free[kStages];  // O of the stage's key tile complete
+    uint64_t kc_full[kStages];  // K' of a stage written (one arrival per converter warp)
+    uint64_t vc_full[kStages];  // V of a stage written
+    uint64_t k_free[kStages];   // S of the stage's key tile complete (both halves)
+    uint64_t v_free[kStages];   // O of it complete (both halves)
+    uint64_t top_full[kTops];   // top written
     uint64_t s_full[2][2];      // [half][buffer]: S complete
-    uint64_t p_full[2][2];      // P written, O rescaled if need be (128 arrivals)
+    uint64_t p_full[2][2];      // P written, O rescaled if need be (one arrival per warp)
     uint64_t o_full[2][2];      // O of that key tile complete
-    uint64_t drain;
+    uint64_t drain[2];
     uint64_t item_full[2];      // two-slot queue of work items
     uint64_t item_free[2];
-    uint64_t q_full;            // Q of the item written (256 arrivals)
-    int32_t top[kStages];       // A of the stage's key tile
+    uint64_t q_full[2];         // Q of a half of the item written
+    int32_t top[kTops];         // A of a key tile
     uint32_t tmem_base;
     int32_t items[2];
     int32_t abort;
@@ -102,13 +105,13 @@ template <int HD>
 struct Shape {
     static constexpr uint32_t ATOM = kKeys * 128;           // 64 keys x 64 dims of K' or V'
     static constexpr uint32_t TILE = ATOM * (HD / 64);
-    static constexpr uint32_t STAGE = 2 * TILE;
     static constexpr uint32_t Q_ATOM = kHalf * 128;         // 128 rows x 64 dims
     static constexpr uint32_t Q_HALF = Q_ATOM * (HD / 64);
     static constexpr uint32_t OFF_Q = 0;
-    static constexpr uint32_t OFF_KV = 2 * Q_HALF;
+    static constexpr uint32_t OFF_K = 2 * Q_HALF;
+    static constexpr uint32_t OFF_V = OFF_K + kStages * TILE;
     static constexpr uint32_t RAW = 2 * kKeys * HD;         // codes of a key tile
-    static constexpr uint32_t OFF_RAW = OFF_KV + kStages * STAGE;
+    static constexpr uint32_t OFF_RAW = OFF_V + kStages * TILE;
     static constexpr uint32_t OFF_CTL = OFF_RAW + kRaw * RAW;
     static constexpr uint32_t SMEM = OFF_CTL + 512 + 1024;  // + control block + alignment slack
     static_assert(SMEM <= 227u * 1024u, "shared memory");
@@ -118,9 +121,9 @@ struct Shape {
     static constexpr int COPIES = kKeys / STEP;                // per thread and tensor
 };
 
-// Bounded wait that also gives up once another role has aborted.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Bounded wait that also gives up once another role has aborted. Only its first
+// try is inlined: the roles run beside one another and share the instruction cache.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, Control* ctl) {
     const uint64_t t0 = global_ns();
     for (;;) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -131,6 +134,9 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Co
             return false;
         }
     }
+}
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl) {
+    return mbar_try_wait(bar, parity) || wait_long(bar, parity, ctl);
 }
 
 __device__ __forceinline__ float ex2_ftz(float x) {
@@ -248,7 +254,8 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     unsigned char* base = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sQ = base + S::OFF_Q;
-    unsigned char* sKV = base + S::OFF_KV;
+    unsigned char* sK = base + S::OFF_K;
+    unsigned char* sV = base + S::OFF_V;
     Control* ctl = reinterpret_cast<Control*>(base + S::OFF_CTL);
     const int tid = threadIdx.x;
     const int warp = tid >> 5;
@@ -256,21 +263,23 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&ctl->kc_full[i], kConvThreads);
-            mbar_init(&ctl->vc_full[i], kConvThreads);
-            mbar_init(&ctl->st_free[i], 1);
+            mbar_init(&ctl->kc_full[i], kConvThreads / 32);
+            mbar_init(&ctl->vc_full[i], kConvThreads / 32);
+            mbar_init(&ctl->k_free[i], 2);
+            mbar_init(&ctl->v_free[i], 2);
         }
+        for (int i = 0; i < kTops; ++i) mbar_init(&ctl->top_full[i], 1);
         for (int i = 0; i < 2; ++i) {
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&ctl->s_full[i][b], 1);
-                mbar_init(&ctl->p_full[i][b], kHalf);
+                mbar_init(&ctl->p_full[i][b], kHalf / 32);
                 mbar_init(&ctl->o_full[i][b], 1);
             }
             mbar_init(&ctl->item_full[i], 1);
+            mbar_init(&ctl->drain[i], 1);
+            mbar_init(&ctl->q_full[i], kHalf / 32);
             mbar_init(&ctl->item_free[i], kItemReaders);
         }
-        mbar_init(&ctl->drain, 1);
-        mbar_init(&ctl->q_full, kRows);
         ctl->abort = 0;
     }
     fence_barrier_init();
@@ -293,6 +302,11 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
         return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl));
+    };
+    // One arrival for the warp, after all its lanes' writes (each fenced by its lane).
+    auto warp_arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
     };
     // Work items: the first converter warp takes each from the global cursor and
     // publishes it in queue slot j % 2; every other warp reads the items in order
@@ -404,7 +418,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 }
                 tc::fence_async_smem();
             }
-            mbar_arrive(&ctl->q_full);
+            warp_arrive(&ctl->q_full[half]);
             const int pos = first_pos + (item.row0 + min(half * kHalf + r, nrows - 1)) / p.group;
             float m = -INFINITY, l = 0.f;
             bool ok = true;
@@ -412,13 +426,12 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const uint32_t n = n0 + t;
                 const uint32_t hn = hn0 + t;
                 const uint32_t b = hn & 1u;
-                // (the stage's own barrier orders its exponents)
-                if (!wait_all(&ctl->kc_full[n % kStages], (n / kStages) & 1u) ||
+                if (!wait_all(&ctl->top_full[n % kTops], (n / kTops) & 1u) ||
                     !wait_all(&ctl->s_full[half][b], (hn >> 1) & 1u)) {
                     ok = false;
                     break;
                 }
-                const int A = *reinterpret_cast<const volatile int32_t*>(&ctl->top[n % kStages]);
+                const int A = *reinterpret_cast<const volatile int32_t*>(&ctl->top[n % kTops]);
                 tc::fence_after_sync();
                 const uint32_t tS = tmem + 128u * half + 64u * b + lane_off;
                 float sc[kKeys];
@@ -486,7 +499,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 l = fmaf(l, alpha, (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
-                mbar_arrive(&ctl->p_full[half][b]);
+                warp_arrive(&ctl->p_full[half][b]);
             }
             if (ok && half < halves) {
                 const uint32_t hn = hn0 + ntiles - 1;
@@ -660,11 +673,14 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 // E4M3 above 2^7 would need a factor beyond bf16's range: the rest of
                 // it is a second factor, which almost no tile has
                 const bool large = kBias > 0 && __any_sync(0xffffffffu, max(e.v[0], e.v[1]) > 7);
-                if (n >= uint32_t(kStages) && !wait_all(&ctl->st_free[st], (n / kStages - 1) & 1u)) break;
+                if (n >= uint32_t(kStages) && !wait_all(&ctl->k_free[st], (n / kStages - 1) & 1u)) break;
                 kv8_copy_wait<2>();  // this tile's pieces, which this thread copied
                 const unsigned char* raw = sRaw + raw_slot * S::RAW + ct * 16;
-                unsigned char* stage = sKV + st * S::STAGE;
-                if (ct == 0) ctl->top[st] = A;
+                unsigned char* stage = sK + st * S::TILE;
+                if (ct == 0) {
+                    ctl->top[n % kTops] = A;
+                    mbar_arrive(&ctl->top_full[n % kTops]);
+                }
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
                     const int el = S::STEP * i / 32;
@@ -680,8 +696,9 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
                 }
                 tc::fence_async_smem();
-                mbar_arrive(&ctl->kc_full[st]);
-                stage += S::TILE;
+                warp_arrive(&ctl->kc_full[st]);
+                if (n >= uint32_t(kStages) && !wait_all(&ctl->v_free[st], (n / kStages - 1) & 1u)) break;
+                stage = sV + st * S::TILE;
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
                     const int el = S::STEP * i / 32;
@@ -707,7 +724,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
                 }
                 tc::fence_async_smem();
-                mbar_arrive(&ctl->vc_full[st]);
+                warp_arrive(&ctl->vc_full[st]);
                 raw_slot = raw_slot + 1 < kRaw ? raw_slot + 1 : 0;
             }
             done(job);
@@ -716,81 +733,95 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     } else {
         // ------------------------------------------------------------------- MMAs
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-        // operand descriptors, built once: offsets are added to their address field
-        // (16-byte units), since one thread's instructions pace the MMAs
-        // what they are built from is made warp-uniform, so that it lives in uniform
-        // registers, where the instructions take it from
+        // One warp issues a half's MMAs. Its own instructions pace it (a few dependent
+        // ones cost as much as an MMA), so what they need is built once and stepped:
+        // descriptors, barrier addresses, and stage and phase of the next O and S. All
+        // of it is warp-uniform and lives in uniform registers, where the
+        // instructions take it from.
         auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
-        const uint32_t utmem = uniform(tmem);
-        const uint64_t q_desc = tc::sw128_desc(uniform(smem_addr(sQ)), 16, 1024);
-        const uint64_t k_desc = tc::sw128_desc(uniform(smem_addr(sKV)), 16, 1024);
-        const uint64_t v_desc = tc::sw128_desc(uniform(smem_addr(sKV + S::TILE)), S::ATOM, 1024);
-        for (uint32_t j = 0; warp == kMmaWarp; ++j) {
+        const uint32_t i = uniform(warp - kMmaWarp);
+        const uint64_t q_desc = tc::sw128_desc(uniform(smem_addr(sQ)) + i * S::Q_HALF, 16, 1024);
+        const uint64_t k_desc = tc::sw128_desc(uniform(smem_addr(sK)), 16, 1024);
+        const uint64_t v_desc = tc::sw128_desc(uniform(smem_addr(sV)), S::ATOM, 1024);
+        const uint32_t tS = uniform(tmem) + 128u * i;
+        const uint32_t tO = uniform(tmem) + 256u + 128u * i;
+        auto both = [&](uint64_t* x, uint32_t px, uint64_t* y, uint32_t py) -> bool {
+            return __all_sync(0xffffffffu, wait_or_abort(x, px, ctl) && wait_or_abort(y, py, ctl));
+        };
+        uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;  // stage and phase of the next S and O
+        uint32_t s_n = 0, o_n = 0;                        // S and O of this half so far
+        for (uint32_t j = 0; warp < kMmaWarp + 2; ++j) {
             const int it = next_item(j);
             if (it < 0) break;
             const Job job = job_of(it);
-            const int ntiles = int(uniform(uint32_t(job.ntiles))), halves = int(uniform(uint32_t(job.halves)));
-            const uint32_t n0 = uniform(seq), h1 = uniform(seq1);
-            auto issue_s = [&](uint32_t n) -> bool {
-                if (!wait_all(&ctl->kc_full[n % kStages], (n / kStages) & 1u)) return false;
-                // S goes where P of the key tile two back was: its O must be complete
-                for (int i = 0; i < halves; ++i) {
-                    const uint32_t hn = (i ? h1 : n0) + (n - n0);
-                    if (n - n0 >= 2 && !wait_all(&ctl->o_full[i][hn & 1u], ((hn - 2) >> 1) & 1u)) return false;
-                }
-                if (tc::elect_one()) {
-                    tc::fence_after_sync();
-                    const uint64_t kd = k_desc + n % kStages * (S::STAGE >> 4);
-                    for (int i = 0; i < halves; ++i) {
-                        const uint32_t hn = (i ? h1 : n0) + (n - n0);
-                        const uint32_t d = utmem + 128u * i + 64u * (hn & 1u);
-                        const uint64_t qd = q_desc + i * (S::Q_HALF >> 4);
+            const int ntiles = int(uniform(uint32_t(job.ntiles)));
+            const bool on = uniform(uint32_t(job.halves)) > i;
+            // t < 0: the first two S. Then O(t) and the S that takes its P's place; the
+            // softmax works on S(t + 1) meanwhile.
+            bool ok = !on || wait_all(&ctl->q_full[i], j & 1u);
+            for (int t = -2; ok && t < ntiles; ++t) {
+                if (t >= 0) {
+                    const uint32_t b = o_n & 1u;
+                    ok = on ? both(&ctl->vc_full[v_st], v_ph, &ctl->p_full[i][b], (o_n >> 1) & 1u)
+                            : wait_all(&ctl->vc_full[v_st], v_ph);
+                    if (!ok) break;
+                    if (tc::elect_one()) {
+                        if (on) {
+                            tc::fence_after_sync();
+                            const uint64_t vd = v_desc + v_st * (S::TILE >> 4);
+                            const uint32_t pb = tS + 64u * b;
 #pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) {
-                            tc::mma_f16(d, qd + ((k >> 2) * (S::Q_ATOM >> 4) + (k & 3) * 2),
-                                        kd + ((k >> 2) * (S::ATOM >> 4) + (k & 3) * 2), kIdescS, k > 0);
+                            for (int k = 0; k < kKeys / 16; ++k) {
+                                const uint64_t v = vd + k * (2048 >> 4);
+                                tc::mma_f16_ts(tO, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
+                                if constexpr (NP == 2) tc::mma_f16_ts(tO, pb + 32u + 8u * k, v, kIdescO, true);
+                            }
+                            tc::commit(&ctl->o_full[i][b]);
+                            tc::commit(&ctl->v_free[v_st]);
+                        } else {
+                            mbar_arrive(&ctl->v_free[v_st]);
                         }
-                        tc::commit(&ctl->s_full[i][hn & 1u]);
-                    }
-                }
-                issued_mma = true;
-                __syncwarp();
-                return true;
-            };
-            bool ok = wait_all(&ctl->q_full, j & 1u) && issue_s(n0);
-            for (int t = 0; ok && t < ntiles; ++t) {
-                const uint32_t n = n0 + t;
-                if (t + 1 < ntiles && !issue_s(n + 1)) break;
-                ok = wait_all(&ctl->vc_full[n % kStages], (n / kStages) & 1u);
-                for (int i = 0; ok && i < halves; ++i) {
-                    const uint32_t hn = (i ? h1 : n0) + t;
-                    ok = wait_all(&ctl->p_full[i][hn & 1u], (hn >> 1) & 1u);
-                    if (ok && tc::elect_one()) {
-                        tc::fence_after_sync();
-                        const uint64_t vd = v_desc + n % kStages * (S::STAGE >> 4);
-                        const uint32_t pb = utmem + 128u * i + 64u * (hn & 1u);
-                        const uint32_t d = utmem + 256u + 128u * i;
-#pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k) {
-                            const uint64_t v = vd + k * (2048 >> 4);
-                            tc::mma_f16_ts(d, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
-                            if constexpr (NP == 2) tc::mma_f16_ts(d, pb + 32u + 8u * k, v, kIdescO, true);
-                        }
-                        tc::commit(&ctl->o_full[i][hn & 1u]);
-                        if (i + 1 == halves) tc::commit(&ctl->st_free[n % kStages]);
                     }
                     __syncwarp();
+                    if (++v_st == kStages) v_st = 0, v_ph ^= 1u;
+                    o_n += on;
+                }
+                if (t + 2 < ntiles) {
+                    const uint32_t b = s_n & 1u;
+                    // the P in this S's place is read once O(t) completes
+                    ok = on && t >= 0 ? both(&ctl->kc_full[k_st], k_ph, &ctl->o_full[i][b], ((s_n - 2) >> 1) & 1u)
+                                      : wait_all(&ctl->kc_full[k_st], k_ph);
+                    if (!ok) break;
+                    if (tc::elect_one()) {
+                        if (on) {
+                            tc::fence_after_sync();
+                            const uint64_t kd = k_desc + k_st * (S::TILE >> 4);
+                            const uint32_t d = tS + 64u * b;
+#pragma unroll
+                            for (int k = 0; k < HD / 16; ++k) {
+                                tc::mma_f16(d, q_desc + ((k >> 2) * (S::Q_ATOM >> 4) + (k & 3) * 2),
+                                            kd + ((k >> 2) * (S::ATOM >> 4) + (k & 3) * 2), kIdescS, k > 0);
+                            }
+                            tc::commit(&ctl->s_full[i][b]);
+                            tc::commit(&ctl->k_free[k_st]);
+                        } else {
+                            mbar_arrive(&ctl->k_free[k_st]);
+                        }
+                    }
+                    issued_mma = true;
+                    __syncwarp();
+                    if (++k_st == kStages) k_st = 0, k_ph ^= 1u;
+                    s_n += on;
                 }
             }
-            done(job);
         }
     }
 
     // Teardown: on an abort, let this CTA's MMAs finish (bounded) before its
     // shared memory and TMEM are released.
-    if (warp == kMmaWarp && issued_mma && tc::elect_one()) {
-        tc::commit(&ctl->drain);
-        mbar_wait(&ctl->drain, 0, kStatusInKv8Tc);
+    if (issued_mma && tc::elect_one()) {
+        tc::commit(&ctl->drain[warp - kMmaWarp]);
+        mbar_wait(&ctl->drain[warp - kMmaWarp], 0, kStatusInKv8Tc);
     }
     tc::fence_before_sync();
     __syncthreads();
