@@ -24,6 +24,10 @@ enum : uint32_t {
     kStatusInKv8Tc = 1u << 16,
 };
 
+// A file compiled on its own (NVLLM_WHOLE_PROGRAM, for the register splits that
+// relocatable code does not allow) cannot name them: its kernels take the status
+// word's address.
+#ifndef NVLLM_WHOLE_PROGRAM
 extern __device__ uint32_t g_status;
 // Where the first bounded wait that gave up was: {site bits, where code (set by
 // the kernel: role, barrier, unit), block index, raw mbarrier word}; word 0 is 0
@@ -52,6 +56,7 @@ __device__ __forceinline__ void record_flag_timeout(uint32_t site, uint32_t targ
         __threadfence();
     }
 }
+#endif  // NVLLM_WHOLE_PROGRAM
 
 // Geometry of the reference arena [num_blocks, L, B, H*hd] in floats.
 struct ArenaGeom {
@@ -114,6 +119,7 @@ __device__ __forceinline__ uint64_t global_ns() {
 // launch ends by itself.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 
+#ifndef NVLLM_WHOLE_PROGRAM
 // Bounded wait: returns false (and raises kStatusTimeout | site) if the phase
 // does not complete within kWaitLimitNs.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t site = 0) {
@@ -127,6 +133,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
         }
     }
 }
+#endif  // NVLLM_WHOLE_PROGRAM
 
 // ---- bulk async copy global -> shared (TMA, no multicast) -----------------
 // dst and src 16-byte aligned, bytes a multiple of 16.

@@ -61,6 +61,7 @@ struct Kv8AttnParams {
     int32_t window;
     int32_t sinks;
     float qk_scale_log2;  // softmax scale * log2(e)
+    uint32_t* status;     // the device status word (whole-program kernels)
 };
 
 // ---- work list ---------------------------------------------------------------

@@ -17,20 +17,20 @@
 // that off by 2^-36 of the largest. P is rounded to bf16, half a step of which is
 // the output's own; for fp16 rows, whose step is finer, P is two bf16 terms.
 //
-// One CTA per SM, 16 warps in 4 warpgroups:
+// One CTA per SM, 20 warps in 5 warpgroups:
 //   warps 0-3, 4-7  softmax of the tile's first and second 128 rows: a thread owns
 //                   a row and its TMEM lane. Reads S, masks ragged tiles, P goes
 //                   back over S as the next product's A operand; O is rescaled
 //                   only when m moves by more than kMargin (rarely).
-//   warps 12, 13    MMAs of the first and second half, one lane each: O(n) += P(n)
+//   warps 8-15      converters: 16-byte pieces of codes to 16-bit floats, into a ring
+//                   of three stages in the MMA's 128-byte swizzle.
+//   warps 16, 17    MMAs of the first and second half, one lane each: O(n) += P(n)
 //                   V(n), then S(n+2) in P's place, while the softmax works on
-//                   S(n+1). Their warpgroup (two more warps do nothing) gives its
-//                   registers to the others.
-//   warps 8-11      converters: 16-byte pieces of codes by asynchronous copies two
-//                   key tiles ahead (block ids three ahead) into a place of the
-//                   thread's own, so that no one else waits for them, then as
-//                   16-bit floats into a ring of three stages in the MMA's
-//                   128-byte swizzle; rows that no query of the tile sees are 0.
+//                   S(n+1).
+//   warps 18, 19    loaders of K and of V: block ids, codes by asynchronous copies
+//                   into a ring of three tiles, and the rows' factors from their
+//                   exponents; rows that no query of the tile sees are 0.
+// The last three warpgroups give registers to the softmax.
 // TMEM (512 columns): S of half i, buffer b at 128 i + 64 b, O of half i at 256 +
 // 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
 // special function units, as many as the products take on the tensor cores at
@@ -51,20 +51,22 @@ constexpr int kHalf = 128;           // rows of a half (TMEM lanes)
 constexpr int kRows = 2 * kHalf;     // rows of a tile
 constexpr int kKeys = 64;            // keys of a key tile
 constexpr int kStages = 3;
-constexpr int kTops = 8;             // more than the converters can be ahead of the softmax
+constexpr int kTops = 16;            // more tiles than K's loader can be ahead of the softmax (8)
 constexpr int kRaw = 3;              // key tiles of codes on their way or landed
 constexpr int kConvWarp0 = 8;
-constexpr int kConvThreads = 128;
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 512;
-constexpr int kItemReaders = kMmaWarp + 1;  // every working warp but the first converter
-// Registers a thread: 128 at launch (65536 / 512). The MMA's warpgroup falls to 40,
-// which frees 88 x 128; the two softmax warpgroups rise to 160 and the converters
-// to 152, which takes (32 + 32 + 24) x 128.
-constexpr int kMmaRegs = 40;
-constexpr int kSoftmaxRegs = 160;
-constexpr int kConvRegs = 152;
-static_assert(2 * kSoftmaxRegs + kConvRegs + kMmaRegs <= 4 * 128, "register split");
+constexpr int kConvWarps = 8;
+constexpr int kMmaWarp = 16;
+constexpr int kLoadWarp = 18;  // K's loader, then V's
+constexpr int kThreads = 640;
+constexpr int kItemReaders = kThreads / 32 - 1;  // every warp but K's loader
+// Registers a thread: 96 at launch (65536 / 640). The converters' two warpgroups
+// fall to 64 and the last to 64, the two softmax warpgroups rise to 144:
+// 2 x 144 + 2 x 64 + 64 = 5 x 96.
+constexpr int kLaunchRegs = 96;
+constexpr int kSoftmaxRegs = 144;
+constexpr int kConvRegs = 64;
+constexpr int kMmaRegs = 64;
+static_assert(2 * kSoftmaxRegs + 2 * kConvRegs + kMmaRegs <= 5 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr int kSms = 148;
 constexpr float kMargin = 8.0f;
@@ -83,6 +85,8 @@ constexpr uint32_t idesc(int M, int N, bool bf16, bool b_mn) {
 }
 
 struct Control {
+    uint64_t raw_full[2][kRaw]; // [K, V]: codes landed (32 arrivals) and factors written
+    uint64_t raw_free[2][kRaw]; // and read (one arrival per converter warp)
     uint64_t kc_full[kStages];  // K' of a stage written (one arrival per converter warp)
     uint64_t vc_full[kStages];  // V of a stage written
     uint64_t k_free[kStages];   // S of the stage's key tile complete (both halves)
@@ -96,6 +100,7 @@ struct Control {
     uint64_t item_free[2];
     uint64_t q_full[2];         // Q of a half of the item written
     int32_t top[kTops];         // A of a key tile
+    int32_t large[kRaw];        // some V exponent of a key tile is above 7
     uint32_t tmem_base;
     int32_t items[2];
     int32_t abort;
@@ -110,33 +115,32 @@ struct Shape {
     static constexpr uint32_t OFF_Q = 0;
     static constexpr uint32_t OFF_K = 2 * Q_HALF;
     static constexpr uint32_t OFF_V = OFF_K + kStages * TILE;
-    static constexpr uint32_t RAW = 2 * kKeys * HD;         // codes of a key tile
+    static constexpr uint32_t RAW = kKeys * HD;             // codes of a key tile of K or V
     static constexpr uint32_t OFF_RAW = OFF_V + kStages * TILE;
-    static constexpr uint32_t OFF_CTL = OFF_RAW + kRaw * RAW;
-    static constexpr uint32_t SMEM = OFF_CTL + 512 + 1024;  // + control block + alignment slack
+    static constexpr uint32_t OFF_FACTOR = OFF_RAW + 2 * kRaw * RAW;
+    static constexpr uint32_t OFF_CTL = OFF_FACTOR + 2 * kRaw * kKeys * 8;
+    static constexpr uint32_t SMEM = OFF_CTL + 1024 + 1024;  // + control block + alignment slack
     static_assert(SMEM <= 227u * 1024u, "shared memory");
-    static_assert(sizeof(Control) <= 512, "control block");
+    static_assert(sizeof(Control) <= 1024, "control block");
     static constexpr int PIECES = HD / 16;                     // 16-code pieces of a row
-    static constexpr int STEP = kConvThreads / PIECES;         // rows converted at once
-    static constexpr int COPIES = kKeys / STEP;                // per thread and tensor
+    static constexpr int STEP = kConvWarps * 32 / PIECES;      // rows converted at once
+    static constexpr int COPIES = kKeys / STEP;                // pieces per thread and tensor
+    static constexpr int LOAD_STEP = 32 / PIECES;              // rows that a loader copies at once
 };
 
-// Bounded wait that also gives up once another role has aborted. Only its first
-// try is inlined: the roles run beside one another and share the instruction cache.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, Control* ctl) {
+// Bounded wait that also gives up once another role has aborted.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl, uint32_t* status) {
+    if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     for (;;) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*reinterpret_cast<volatile int32_t*>(&ctl->abort)) return false;
         if (global_ns() - t0 > kWaitLimitNs) {
-            raise_status(kStatusTimeout | kStatusInKv8Tc);
+            atomicOr(status, kStatusTimeout | kStatusInKv8Tc);
             atomicExch(&ctl->abort, 1);
             return false;
         }
     }
-}
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl) {
-    return mbar_try_wait(bar, parity) || wait_long(bar, parity, ctl);
 }
 
 __device__ __forceinline__ float ex2_ftz(float x) {
@@ -256,6 +260,8 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     unsigned char* sQ = base + S::OFF_Q;
     unsigned char* sK = base + S::OFF_K;
     unsigned char* sV = base + S::OFF_V;
+    unsigned char* sRaw = base + S::OFF_RAW;  // [K, V][slot][row][HD]
+    uint32_t* sFactor = reinterpret_cast<uint32_t*>(base + S::OFF_FACTOR);  // [K, V][slot][row][2]
     Control* ctl = reinterpret_cast<Control*>(base + S::OFF_CTL);
     const int tid = threadIdx.x;
     const int warp = tid >> 5;
@@ -263,10 +269,14 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&ctl->kc_full[i], kConvThreads / 32);
-            mbar_init(&ctl->vc_full[i], kConvThreads / 32);
+            mbar_init(&ctl->kc_full[i], kConvWarps);
+            mbar_init(&ctl->vc_full[i], kConvWarps);
             mbar_init(&ctl->k_free[i], 2);
             mbar_init(&ctl->v_free[i], 2);
+        }
+        for (int i = 0; i < 2 * kRaw; ++i) {
+            mbar_init(&ctl->raw_full[0][i], 33);
+            mbar_init(&ctl->raw_free[0][i], kConvWarps);
         }
         for (int i = 0; i < kTops; ++i) mbar_init(&ctl->top_full[i], 1);
         for (int i = 0; i < 2; ++i) {
@@ -301,20 +311,20 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     bool issued_mma = false;   // MMA warp
 
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl));
+        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl, p.status));
     };
     // One arrival for the warp, after all its lanes' writes (each fenced by its lane).
     auto warp_arrive = [&](uint64_t* bar) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
     };
-    // Work items: the first converter warp takes each from the global cursor and
+    // Work items: K's loader takes each from the global cursor and
     // publishes it in queue slot j % 2; every other warp reads the items in order
     // and frees the slot. -1 ends the loop. No role waits for the others at an
     // item's end.
     auto publish = [&](uint32_t j, int it) -> bool {
         const uint32_t slot = j & 1u;
-        if (j >= 2 && !wait_or_abort(&ctl->item_free[slot], ((j >> 1) - 1) & 1u, ctl)) return false;
+        if (j >= 2 && !wait_or_abort(&ctl->item_free[slot], ((j >> 1) - 1) & 1u, ctl, p.status)) return false;
         ctl->items[slot] = it;
         mbar_arrive(&ctl->item_full[slot]);
         return true;
@@ -330,7 +340,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 
     auto next_item = [&](uint32_t j) -> int {
         int it = -1;
-        if (warp == kConvWarp0) {
+        if (warp == kLoadWarp) {
             if (lane == 0) {
                 if (!*reinterpret_cast<volatile int32_t*>(&ctl->abort)) {
                     it = atomicAdd(&w.counters->next, 1);
@@ -549,13 +559,10 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
         }
     } else if (warp < kMmaWarp) {
         // ------------------------------------------------------------- converters
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
         const int ct = tid - 32 * kConvWarp0;
         const int piece = ct % S::PIECES;
         const int row0 = ct / S::PIECES;
-        unsigned char* sRaw = base + S::OFF_RAW;
-        const uint32_t raw_addr = smem_addr(sRaw) + ct * 16;
-        uint32_t raw_slot = 0;  // of the next tile to convert
         // Where the thread's piece goes: atom piece / 4, two 16-byte chunks swizzled by
         // the row (STEP is a multiple of 8: the same for all its rows). Pieces of the
         // second atom write theirs in the other order, so that the 8 lanes of a row
@@ -564,155 +571,68 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
         const uint32_t put_row = (piece >> 2) * S::ATOM + row0 * 128;
         const uint32_t put0 = put_row + (((piece & 3) * 2 + swap) ^ (row0 & 7)) * 16;
         const uint32_t put1 = put_row + (((piece & 3) * 2 + 1 - swap) ^ (row0 & 7)) * 16;
+        const unsigned char* my_raw = sRaw + ct * 16;
+        uint32_t slot = 0, slot_ph = 0;  // of the next tile's codes
+        uint32_t st = 0, st_ph = 1;      // of the next stage, and the phase that frees it
         for (uint32_t j = 0;; ++j) {
             const int it = next_item(j);
             if (it < 0) break;
             const Job job = job_of(it);
-            const Kv8Item& item = job.item;
-            const int h = job.h, ntiles = job.ntiles, pos_lo = job.pos_lo, pos_hi = job.pos_hi;
-            const uint32_t n0 = seq;
-            const int32_t* table = p.block_tables + int64_t(item.seq) * p.max_blocks;
-            const int64_t column = int64_t(h) * HD + piece * 16;
-            const int64_t exp_head = int64_t(h) * p.a.block_size;
-            // lane l finds positions l and l + 32 of a tile: the table's entry (kNone
-            // where no row sees) and the slot
-            constexpr int kNone = INT32_MIN;
-            struct Where {
-                int blk[2], in[2];
-            };
-            auto find = [&](int c) -> Where {
-                Where x;
-                const int kbase = kv8_chunk(item, c) * kKeys + lane;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int pos = kbase + 32 * i;
-                    x.blk[i] = kNone;
-                    x.in[i] = 0;
-                    if (c < item.c1 && pos <= pos_hi &&
-                        (p.window <= 0 || pos > pos_lo - p.window || pos < p.sinks)) {
-                        int entry;
-                        kv8_place(p.a, pos, entry, x.in[i]);
-                        x.blk[i] = __ldg(table + entry);
-                    }
-                }
-                return x;
-            };
-            auto check = [&](Where& x) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (x.blk[i] != kNone && (x.blk[i] < 0 || x.blk[i] >= p.a.num_blocks)) {
-                        raise_status(kStatusBounds);
-                        x.blk[i] = kNone;
-                    }
-                }
-            };
-            struct Exps {
-                int k[2], v[2];  // of positions l, l + 32
-            };
-            auto load_exps = [&](const Where& x) -> Exps {
-                Exps e;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    e.k[i] = e.v[i] = -1000;  // nothing there
-                    if (x.blk[i] >= 0) {
-                        const int64_t at = int64_t(x.blk[i]) * p.a.exp_block_stride + exp_head + x.in[i];
-                        e.k[i] = __ldg(p.a.k_exps + at);
-                        e.v[i] = __ldg(p.a.v_exps + at);
-                    }
-                }
-                return e;
-            };
-            // the thread's rows of a tile are row0 + STEP i; row r's finder is lane
-            // r % 32, element r / 32, which depends on i alone
-            auto copy = [&](const Where& x, uint32_t slot) {
-                const uint32_t dst = raw_addr + slot * S::RAW;
+            const int ntiles = job.ntiles;
+            bool ok = true;
+            for (int t = 0; ok && t < ntiles; ++t) {
+                // K'
+                ok = wait_all(&ctl->raw_full[0][slot], slot_ph);
+                if (!ok) break;
+                uint4 x[S::COPIES];
+                uint2 f[S::COPIES];
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
-                    constexpr int kHalfRows = 32;
-                    const int el = S::STEP * i / kHalfRows;
-                    const int from = (row0 + S::STEP * i) & 31;
-                    const int blk = __shfl_sync(0xffffffffu, x.blk[el], from);
-                    const int in = __shfl_sync(0xffffffffu, x.in[el], from);
-                    const int64_t at = int64_t(max(blk, 0)) * p.a.block_stride + int64_t(in) * p.a.row + column;
-                    kv8_copy16(dst + i * 2 * kConvThreads * 16, p.a.k_codes + at, blk >= 0);
-                    kv8_copy16(dst + (2 * i + 1) * kConvThreads * 16, p.a.v_codes + at, blk >= 0);
+                    x[i] = *reinterpret_cast<const uint4*>(my_raw + slot * S::RAW + i * S::STEP * HD);
+                    f[i].x = sFactor[(slot * kKeys + row0 + S::STEP * i) * 2];
                 }
-            };
-            // copies two tiles ahead, exponents one, block ids three
-            Where w1 = find(item.c0), w2 = find(item.c0 + 1), w3 = find(item.c0 + 2);
-            check(w1);
-            copy(w1, raw_slot);
-            kv8_copy_commit();
-            Exps e1 = load_exps(w1);
-            check(w2);
-            if (ntiles > 1) copy(w2, raw_slot + 1 < kRaw ? raw_slot + 1 : raw_slot + 1 - kRaw);
-            kv8_copy_commit();
-            w1 = w2;
-            for (int t = 0; t < ntiles; ++t) {
-                const uint32_t n = n0 + t;
-                const uint32_t st = n % kStages;
-                check(w3);
-                if (t + 2 < ntiles) copy(w3, raw_slot + 2 < kRaw ? raw_slot + 2 : raw_slot + 2 - kRaw);
-                kv8_copy_commit();
-                const Exps e = e1;
-                e1 = load_exps(w1);
-                w1 = w3;
-                w3 = find(item.c0 + t + 3);
-                const int A = max(__reduce_max_sync(0xffffffffu, max(e.k[0], e.k[1])), kKv8MinExp);
-                // the factors of the lane's two positions, as pairs
-                constexpr int kBias = kFormat == NVLLM_KV8_E4M3 ? 120 : 0;
-                uint32_t fk[2], fv[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const __half2 a = half_power(e.k[i] - A + U);
-                    const __nv_bfloat162 b =
-                        __float2bfloat162_rn(exp2_int(min(max(e.v[i], -126) + kBias, 127)));
-                    fk[i] = *reinterpret_cast<const uint32_t*>(&a);
-                    fv[i] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-                // E4M3 above 2^7 would need a factor beyond bf16's range: the rest of
-                // it is a second factor, which almost no tile has
-                const bool large = kBias > 0 && __any_sync(0xffffffffu, max(e.v[0], e.v[1]) > 7);
-                if (n >= uint32_t(kStages) && !wait_all(&ctl->k_free[st], (n / kStages - 1) & 1u)) break;
-                kv8_copy_wait<2>();  // this tile's pieces, which this thread copied
-                const unsigned char* raw = sRaw + raw_slot * S::RAW + ct * 16;
+                warp_arrive(&ctl->raw_free[0][slot]);
+                // a stage's first use waits for nothing (the phase before the first)
+                ok = wait_all(&ctl->k_free[st], st_ph);
+                if (!ok) break;
                 unsigned char* stage = sK + st * S::TILE;
-                if (ct == 0) {
-                    ctl->top[n % kTops] = A;
-                    mbar_arrive(&ctl->top_full[n % kTops]);
-                }
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
-                    const int el = S::STEP * i / 32;
-                    const uint32_t f = __shfl_sync(0xffffffffu, fk[el], (row0 + S::STEP * i) & 31);
-                    const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
-                    const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 2 * kConvThreads * 16);
+                    const __half2 f2 = *reinterpret_cast<const __half2*>(&f[i].x);
                     uint4 a, b;
-                    scaled_half4<kFormat>(x.x, f2, a.x, a.y);
-                    scaled_half4<kFormat>(x.y, f2, a.z, a.w);
-                    scaled_half4<kFormat>(x.z, f2, b.x, b.y);
-                    scaled_half4<kFormat>(x.w, f2, b.z, b.w);
+                    scaled_half4<kFormat>(x[i].x, f2, a.x, a.y);
+                    scaled_half4<kFormat>(x[i].y, f2, a.z, a.w);
+                    scaled_half4<kFormat>(x[i].z, f2, b.x, b.y);
+                    scaled_half4<kFormat>(x[i].w, f2, b.z, b.w);
                     *reinterpret_cast<uint4*>(stage + put0 + i * S::STEP * 128) = swap ? b : a;
                     *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
                 }
                 tc::fence_async_smem();
                 warp_arrive(&ctl->kc_full[st]);
-                if (n >= uint32_t(kStages) && !wait_all(&ctl->v_free[st], (n / kStages - 1) & 1u)) break;
+                // V
+                ok = wait_all(&ctl->raw_full[1][slot], slot_ph);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < S::COPIES; ++i) {
+                    x[i] = *reinterpret_cast<const uint4*>(my_raw + (kRaw + slot) * S::RAW + i * S::STEP * HD);
+                    f[i] = *reinterpret_cast<const uint2*>(
+                        sFactor + ((kRaw + slot) * kKeys + row0 + S::STEP * i) * 2);
+                }
+                const bool large = ctl->large[slot];
+                warp_arrive(&ctl->raw_free[1][slot]);
+                ok = wait_all(&ctl->v_free[st], st_ph);
+                if (!ok) break;
                 stage = sV + st * S::TILE;
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
-                    const int el = S::STEP * i / 32;
-                    const uint32_t f = __shfl_sync(0xffffffffu, fv[el], (row0 + S::STEP * i) & 31);
-                    const __nv_bfloat162 f2 = *reinterpret_cast<const __nv_bfloat162*>(&f);
-                    const uint4 x = *reinterpret_cast<const uint4*>(raw + (2 * i + 1) * kConvThreads * 16);
+                    const __nv_bfloat162 f2 = *reinterpret_cast<const __nv_bfloat162*>(&f[i].x);
                     uint32_t o[8];
-                    scaled_bf16x4<kFormat>(x.x, f2, o[0], o[1]);
-                    scaled_bf16x4<kFormat>(x.y, f2, o[2], o[3]);
-                    scaled_bf16x4<kFormat>(x.z, f2, o[4], o[5]);
-                    scaled_bf16x4<kFormat>(x.w, f2, o[6], o[7]);
+                    scaled_bf16x4<kFormat>(x[i].x, f2, o[0], o[1]);
+                    scaled_bf16x4<kFormat>(x[i].y, f2, o[2], o[3]);
+                    scaled_bf16x4<kFormat>(x[i].z, f2, o[4], o[5]);
+                    scaled_bf16x4<kFormat>(x[i].w, f2, o[6], o[7]);
                     if (large) {
-                        const int ev = __shfl_sync(0xffffffffu, e.v[el], (row0 + S::STEP * i) & 31);
-                        const __nv_bfloat162 g = __float2bfloat162_rn(exp2_int(max(ev - 7, 0)));
+                        const __nv_bfloat162 g = *reinterpret_cast<const __nv_bfloat162*>(&f[i].y);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&o[k]), g);
@@ -725,93 +645,224 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 }
                 tc::fence_async_smem();
                 warp_arrive(&ctl->vc_full[st]);
-                raw_slot = raw_slot + 1 < kRaw ? raw_slot + 1 : 0;
+                if (++slot == kRaw) slot = 0, slot_ph ^= 1u;
+                if (++st == kStages) st = 0, st_ph ^= 1u;
             }
-            done(job);
         }
-        kv8_copy_wait<0>();
     } else {
-        // ------------------------------------------------------------------- MMAs
+        // one instruction for the whole warpgroup, before its roles part
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-        // One warp issues a half's MMAs. Its own instructions pace it (a few dependent
-        // ones cost as much as an MMA), so what they need is built once and stepped:
-        // descriptors, barrier addresses, and stage and phase of the next O and S. All
-        // of it is warp-uniform and lives in uniform registers, where the
-        // instructions take it from.
-        auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
-        const uint32_t i = uniform(warp - kMmaWarp);
-        const uint64_t q_desc = tc::sw128_desc(uniform(smem_addr(sQ)) + i * S::Q_HALF, 16, 1024);
-        const uint64_t k_desc = tc::sw128_desc(uniform(smem_addr(sK)), 16, 1024);
-        const uint64_t v_desc = tc::sw128_desc(uniform(smem_addr(sV)), S::ATOM, 1024);
-        const uint32_t tS = uniform(tmem) + 128u * i;
-        const uint32_t tO = uniform(tmem) + 256u + 128u * i;
-        auto both = [&](uint64_t* x, uint32_t px, uint64_t* y, uint32_t py) -> bool {
-            return __all_sync(0xffffffffu, wait_or_abort(x, px, ctl) && wait_or_abort(y, py, ctl));
-        };
-        uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;  // stage and phase of the next S and O
-        uint32_t s_n = 0, o_n = 0;                        // S and O of this half so far
-        for (uint32_t j = 0; warp < kMmaWarp + 2; ++j) {
-            const int it = next_item(j);
-            if (it < 0) break;
-            const Job job = job_of(it);
-            const int ntiles = int(uniform(uint32_t(job.ntiles)));
-            const bool on = uniform(uint32_t(job.halves)) > i;
-            // t < 0: the first two S. Then O(t) and the S that takes its P's place; the
-            // softmax works on S(t + 1) meanwhile.
-            bool ok = !on || wait_all(&ctl->q_full[i], j & 1u);
-            for (int t = -2; ok && t < ntiles; ++t) {
-                if (t >= 0) {
-                    const uint32_t b = o_n & 1u;
-                    ok = on ? both(&ctl->vc_full[v_st], v_ph, &ctl->p_full[i][b], (o_n >> 1) & 1u)
-                            : wait_all(&ctl->vc_full[v_st], v_ph);
-                    if (!ok) break;
-                    if (tc::elect_one()) {
-                        if (on) {
-                            tc::fence_after_sync();
-                            const uint64_t vd = v_desc + v_st * (S::TILE >> 4);
-                            const uint32_t pb = tS + 64u * b;
+        if (warp >= kLoadWarp) {
+            // ---------------------------------------------------------------- loaders
+            const int kv = warp - kLoadWarp;  // K's or V's
+            const unsigned char* codes = kv ? p.a.v_codes : p.a.k_codes;
+            const int8_t* exps = kv ? p.a.v_exps : p.a.k_exps;
+            const uint32_t raw_addr = smem_addr(sRaw + kv * kRaw * S::RAW) + lane * 16;
+            uint32_t* factor = sFactor + kv * kRaw * kKeys * 2;
+            const int row0 = lane / S::PIECES;
+            uint32_t slot = 0, slot_ph = 1;  // of the next tile, and the phase that frees it
+            for (uint32_t j = 0;; ++j) {
+                const int it = next_item(j);
+                if (it < 0) break;
+                const Job job = job_of(it);
+                const Kv8Item& item = job.item;
+                const int h = job.h, ntiles = job.ntiles, pos_lo = job.pos_lo, pos_hi = job.pos_hi;
+                const uint32_t n0 = seq;
+                const int32_t* table = p.block_tables + int64_t(item.seq) * p.max_blocks;
+                const int64_t column = int64_t(h) * HD + lane % S::PIECES * 16;
+                const int64_t exp_head = int64_t(h) * p.a.block_size;
+                // lane l finds positions l and l + 32 of a tile: the table's entry (kNone
+                // where no row sees) and the slot
+                constexpr int kNone = INT32_MIN;
+                struct Where {
+                    int blk[2], in[2];
+                };
+                auto find = [&](int c) -> Where {
+                    Where x;
+                    const int kbase = kv8_chunk(item, c) * kKeys + lane;
 #pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k) {
-                                const uint64_t v = vd + k * (2048 >> 4);
-                                tc::mma_f16_ts(tO, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
-                                if constexpr (NP == 2) tc::mma_f16_ts(tO, pb + 32u + 8u * k, v, kIdescO, true);
-                            }
-                            tc::commit(&ctl->o_full[i][b]);
-                            tc::commit(&ctl->v_free[v_st]);
-                        } else {
-                            mbar_arrive(&ctl->v_free[v_st]);
+                    for (int i = 0; i < 2; ++i) {
+                        const int pos = kbase + 32 * i;
+                        x.blk[i] = kNone;
+                        x.in[i] = 0;
+                        if (c < item.c1 && pos <= pos_hi &&
+                            (p.window <= 0 || pos > pos_lo - p.window || pos < p.sinks)) {
+                            int entry;
+                            kv8_place(p.a, pos, entry, x.in[i]);
+                            x.blk[i] = __ldg(table + entry);
                         }
                     }
-                    __syncwarp();
-                    if (++v_st == kStages) v_st = 0, v_ph ^= 1u;
-                    o_n += on;
+                    return x;
+                };
+                // The factors of the lane's two positions, from their exponents (-1000:
+                // nothing there): K's against the tile's largest, V's its own, in E4M3 with
+                // the 2^120 that the codes lack. That leaves bf16's range above 2^7: the
+                // rest is a second factor, which almost no tile has.
+                auto write_factors = [&](const int (&e)[2], uint32_t at, uint32_t n) {
+                    uint32_t* dst = factor + (at * kKeys + lane) * 2;
+                    if (kv == 0) {
+                        const int A = max(__reduce_max_sync(0xffffffffu, max(e[0], e[1])), kKv8MinExp);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const __half2 f = half_power(e[i] - A + U);
+                            dst[64 * i] = *reinterpret_cast<const uint32_t*>(&f);
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            ctl->top[n % kTops] = A;
+                            mbar_arrive(&ctl->top_full[n % kTops]);
+                            mbar_arrive(&ctl->raw_full[0][at]);
+                        }
+                    } else {
+                        constexpr int kBias = kFormat == NVLLM_KV8_E4M3 ? 120 : 0;
+                        const bool large = kBias > 0 && __any_sync(0xffffffffu, max(e[0], e[1]) > 7);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const __nv_bfloat162 f =
+                                __float2bfloat162_rn(exp2_int(min(max(e[i], -126) + kBias, 127)));
+                            const __nv_bfloat162 g = __float2bfloat162_rn(exp2_int(max(e[i] - 7, 0)));
+                            dst[64 * i] = *reinterpret_cast<const uint32_t*>(&f);
+                            dst[64 * i + 1] = *reinterpret_cast<const uint32_t*>(&g);
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            ctl->large[at] = large;
+                            mbar_arrive(&ctl->raw_full[1][at]);
+                        }
+                    }
+                };
+                // block ids two tiles ahead; a tile's exponents are used when the next
+                // tile's copies are on their way
+                Where w = find(item.c0), next = find(item.c0 + 1);
+                int e[2] = {0, 0};
+                uint32_t e_at = 0;
+                bool ok = true;
+                for (int t = 0; t < ntiles; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (w.blk[i] != kNone && (w.blk[i] < 0 || w.blk[i] >= p.a.num_blocks)) {
+                            atomicOr(p.status, kStatusBounds);
+                            w.blk[i] = kNone;
+                        }
+                    }
+                    ok = wait_all(&ctl->raw_free[kv][slot], slot_ph);
+                    if (!ok) break;
+                    int64_t off[2];
+                    int en[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        off[i] = w.blk[i] < 0 ? -1 : int64_t(w.blk[i]) * p.a.block_stride + int64_t(w.in[i]) * p.a.row;
+                        en[i] = -1000;
+                        if (w.blk[i] >= 0) {
+                            en[i] = __ldg(exps + int64_t(w.blk[i]) * p.a.exp_block_stride + exp_head + w.in[i]);
+                        }
+                    }
+                    const uint32_t dst = raw_addr + slot * S::RAW;
+#pragma unroll
+                    for (int i = 0; i < kKeys / S::LOAD_STEP; ++i) {
+                        // row r's finder is lane r % 32, element r / 32, which depends on i alone
+                        const int64_t at = __shfl_sync(0xffffffffu, off[S::LOAD_STEP * i / 32],
+                                                       (row0 + S::LOAD_STEP * i) & 31);
+                        kv8_copy16(dst + i * 512, codes + (at < 0 ? 0 : at + column), at >= 0);
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                                     smem_addr(&ctl->raw_full[kv][slot]))
+                                 : "memory");
+                    w = next;
+                    next = find(item.c0 + t + 2);
+                    if (t > 0) write_factors(e, e_at, n0 + t - 1);
+                    e[0] = en[0];
+                    e[1] = en[1];
+                    e_at = slot;
+                    if (++slot == kRaw) slot = 0, slot_ph ^= 1u;
                 }
-                if (t + 2 < ntiles) {
-                    const uint32_t b = s_n & 1u;
-                    // the P in this S's place is read once O(t) completes
-                    ok = on && t >= 0 ? both(&ctl->kc_full[k_st], k_ph, &ctl->o_full[i][b], ((s_n - 2) >> 1) & 1u)
-                                      : wait_all(&ctl->kc_full[k_st], k_ph);
-                    if (!ok) break;
-                    if (tc::elect_one()) {
-                        if (on) {
-                            tc::fence_after_sync();
-                            const uint64_t kd = k_desc + k_st * (S::TILE >> 4);
-                            const uint32_t d = tS + 64u * b;
+                if (ok) write_factors(e, e_at, n0 + ntiles - 1);
+                done(job);
+            }
+            kv8_copy_commit();
+            kv8_copy_wait<0>();
+        } else {
+            // ------------------------------------------------------------------- MMAs
+            // One warp issues a half's MMAs. Its own instructions pace it (a few dependent
+            // ones cost as much as an MMA), so what they need is built once and stepped:
+            // descriptors, barrier addresses, and stage and phase of the next O and S. All
+            // of it is warp-uniform and lives in uniform registers, where the
+            // instructions take it from.
+            auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+            const uint32_t i = uniform(warp - kMmaWarp);
+            const uint64_t q_desc = tc::sw128_desc(uniform(smem_addr(sQ)) + i * S::Q_HALF, 16, 1024);
+            const uint64_t k_desc = tc::sw128_desc(uniform(smem_addr(sK)), 16, 1024);
+            const uint64_t v_desc = tc::sw128_desc(uniform(smem_addr(sV)), S::ATOM, 1024);
+            const uint32_t tS = uniform(tmem) + 128u * i;
+            const uint32_t tO = uniform(tmem) + 256u + 128u * i;
+            auto both = [&](uint64_t* x, uint32_t px, uint64_t* y, uint32_t py) -> bool {
+                return __all_sync(0xffffffffu, wait_or_abort(x, px, ctl, p.status) && wait_or_abort(y, py, ctl, p.status));
+            };
+            uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;  // stage and phase of the next S and O
+            uint32_t s_n = 0, o_n = 0;                        // S and O of this half so far
+            for (uint32_t j = 0;; ++j) {
+                const int it = next_item(j);
+                if (it < 0) break;
+                const Job job = job_of(it);
+                const int ntiles = int(uniform(uint32_t(job.ntiles)));
+                const bool on = uniform(uint32_t(job.halves)) > i;
+                // t < 0: the first two S. Then O(t) and the S that takes its P's place; the
+                // softmax works on S(t + 1) meanwhile.
+                bool ok = !on || wait_all(&ctl->q_full[i], j & 1u);
+                for (int t = -2; ok && t < ntiles; ++t) {
+                    if (t >= 0) {
+                        const uint32_t b = o_n & 1u;
+                        ok = on ? both(&ctl->vc_full[v_st], v_ph, &ctl->p_full[i][b], (o_n >> 1) & 1u)
+                                : wait_all(&ctl->vc_full[v_st], v_ph);
+                        if (!ok) break;
+                        if (tc::elect_one()) {
+                            if (on) {
+                                tc::fence_after_sync();
+                                const uint64_t vd = v_desc + v_st * (S::TILE >> 4);
+                                const uint32_t pb = tS + 64u * b;
 #pragma unroll
-                            for (int k = 0; k < HD / 16; ++k) {
-                                tc::mma_f16(d, q_desc + ((k >> 2) * (S::Q_ATOM >> 4) + (k & 3) * 2),
-                                            kd + ((k >> 2) * (S::ATOM >> 4) + (k & 3) * 2), kIdescS, k > 0);
+                                for (int k = 0; k < kKeys / 16; ++k) {
+                                    const uint64_t v = vd + k * (2048 >> 4);
+                                    tc::mma_f16_ts(tO, pb + 8u * k, v, kIdescO, k > 0 || t > 0);
+                                    if constexpr (NP == 2) tc::mma_f16_ts(tO, pb + 32u + 8u * k, v, kIdescO, true);
+                                }
+                                tc::commit(&ctl->o_full[i][b]);
+                                tc::commit(&ctl->v_free[v_st]);
+                            } else {
+                                mbar_arrive(&ctl->v_free[v_st]);
                             }
-                            tc::commit(&ctl->s_full[i][b]);
-                            tc::commit(&ctl->k_free[k_st]);
-                        } else {
-                            mbar_arrive(&ctl->k_free[k_st]);
                         }
+                        __syncwarp();
+                        if (++v_st == kStages) v_st = 0, v_ph ^= 1u;
+                        o_n += on;
                     }
-                    issued_mma = true;
-                    __syncwarp();
-                    if (++k_st == kStages) k_st = 0, k_ph ^= 1u;
-                    s_n += on;
+                    if (t + 2 < ntiles) {
+                        const uint32_t b = s_n & 1u;
+                        // the P in this S's place is read once O(t) completes
+                        ok = on && t >= 0 ? both(&ctl->kc_full[k_st], k_ph, &ctl->o_full[i][b], ((s_n - 2) >> 1) & 1u)
+                                          : wait_all(&ctl->kc_full[k_st], k_ph);
+                        if (!ok) break;
+                        if (tc::elect_one()) {
+                            if (on) {
+                                tc::fence_after_sync();
+                                const uint64_t kd = k_desc + k_st * (S::TILE >> 4);
+                                const uint32_t d = tS + 64u * b;
+#pragma unroll
+                                for (int k = 0; k < HD / 16; ++k) {
+                                    tc::mma_f16(d, q_desc + ((k >> 2) * (S::Q_ATOM >> 4) + (k & 3) * 2),
+                                                kd + ((k >> 2) * (S::ATOM >> 4) + (k & 3) * 2), kIdescS, k > 0);
+                                }
+                                tc::commit(&ctl->s_full[i][b]);
+                                tc::commit(&ctl->k_free[k_st]);
+                            } else {
+                                mbar_arrive(&ctl->k_free[k_st]);
+                            }
+                        }
+                        issued_mma = true;
+                        __syncwarp();
+                        if (++k_st == kStages) k_st = 0, k_ph ^= 1u;
+                        s_n += on;
+                    }
                 }
             }
         }
@@ -821,7 +872,9 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     // shared memory and TMEM are released.
     if (issued_mma && tc::elect_one()) {
         tc::commit(&ctl->drain[warp - kMmaWarp]);
-        mbar_wait(&ctl->drain[warp - kMmaWarp], 0, kStatusInKv8Tc);
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait(&ctl->drain[warp - kMmaWarp], 0) && global_ns() - t0 < kWaitLimitNs) {
+        }
     }
     tc::fence_before_sync();
     __syncthreads();

@@ -3,7 +3,7 @@
     python -m nvllm.build          (from nano-vllm-cpp26_b200/)
 
 * lib/libnvllm.so: nvcc compiles every csrc/*.cu for sm_100a with relocatable
-  device code and links them; the static CUDA runtime is linked in so the
+  device code (a few as whole programs) and links them; the static CUDA runtime is linked in so the
   library depends only on the driver.
 * lib/libnvllm_host.so: g++ -std=c++23 compiles host/*.cpp (block allocator,
   metadata packer, engine, device model, their C ABI) against libnvllm.so,
@@ -28,6 +28,15 @@ CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++20", "-lineinfo", "-rdc=true", "-Xcompiler", "-fPIC",
               "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]
+# Files whose kernels split registers between warpgroups (setmaxnreg), which ptxas
+# ignores in relocatable code: compiled as whole programs.
+WHOLE_PROGRAM = {"kv8_attention_tc.cu"}
+
+
+def flags_for(src: Path) -> list[str]:
+    if src.name not in WHOLE_PROGRAM:
+        return NVCC_FLAGS
+    return [f for f in NVCC_FLAGS if f != "-rdc=true"] + ["-DNVLLM_WHOLE_PROGRAM"]
 
 
 def nvcc() -> str:
@@ -61,7 +70,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     for src in sources():
         obj = objdir / (src.stem + ".o")
         objs.append(obj)
-        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, f"-I{INCLUDE}", "-c", str(src), "-o", str(obj)]
+        cmd = [nvcc(), *ARCH, *flags_for(src), f"-I{INCLUDE}", "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd))
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
