@@ -149,6 +149,11 @@ __device__ __forceinline__ float ex2_ftz(float x) {
     return y;
 }
 
+// The lowest n of 64 bits (none below 0, all from 64 on).
+__device__ __forceinline__ uint64_t below(int n) {
+    return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+}
+
 // Two floats by one instruction, and the largest of three.
 __device__ __forceinline__ uint64_t pair(float2 a) {
     uint64_t r;
@@ -451,11 +456,15 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const int kbase = kv8_chunk(item, item.c0 + t) * kKeys;
                 if (kbase + kKeys - 1 > pos_lo ||
                     (p.window > 0 && kbase + p.window <= pos_hi && kbase + kKeys > p.sinks)) {
-                    const int low = p.window > 0 ? pos - p.window : -1;
+                    // the tile's keys that the row sees, a bit each: up to its own, and from
+                    // the window's start or before the sinks' end
+                    uint64_t see = below(pos + 1 - kbase);
+                    if (p.window > 0) see &= ~below(pos + 1 - p.window - kbase) | below(p.sinks - kbase);
+                    const uint32_t see_lo = uint32_t(see), see_hi = uint32_t(see >> 32);
 #pragma unroll
-                    for (int k = 0; k < kKeys; ++k) {
-                        const int key = kbase + k;
-                        if (key > pos || (key <= low && key >= p.sinks)) sc[k] = -INFINITY;
+                    for (int k = 0; k < 32; ++k) {
+                        sc[k] = see_lo & (1u << k) ? sc[k] : -INFINITY;
+                        sc[32 + k] = see_hi & (1u << k) ? sc[32 + k] : -INFINITY;
                     }
                 }
                 // a factor above 0 keeps -inf what it is for rows of zeros
