@@ -62,6 +62,7 @@ struct Kv8AttnParams {
     int32_t sinks;
     float qk_scale_log2;  // softmax scale * log2(e)
     uint32_t* status;     // the device status word (whole-program kernels)
+    bool fp16;            // 16-bit rows are fp16, not bf16 (kernels that serve both)
 };
 
 // ---- work list ---------------------------------------------------------------
@@ -107,6 +108,18 @@ struct Kv8Work {
     int32_t snap;      // ranges end where sequences do: no tile is cut
     int32_t merge_grid;  // CTAs of the merge, 0: no tile is ever cut
 };
+
+constexpr int kKv8Sms = 148;
+constexpr int kKv8Sub = 16;  // positions of one MMA tile of the mma.sync kernel
+
+// 16-position tiles per chunk: independent work between a warp's few, long
+// dependences (a maximum over lanes, a rescale), as far as registers go.
+constexpr int kv8_subs(int head_dim, int nq) {
+    return nq > 2 || head_dim == 256 ? 1 : head_dim == 128 || nq == 2 ? 2 : 4;
+}
+
+// Its CTAs per SM, by registers and shared memory.
+constexpr int kv8_resident(int head_dim, int nq) { return head_dim * nq >= 512 || head_dim == 256 ? 2 : 3; }
 
 // Most sequences of a call without a plan (longer batches take several).
 constexpr int kKv8SelfSeqs = 512;
@@ -228,6 +241,11 @@ size_t kv8_attention_workspace(int32_t num_seqs, int32_t max_query_len, int32_t 
                                int32_t num_query_heads, const ArenaGeom& g);
 cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int32_t dtype, int32_t format,
                                  void* workspace, cudaStream_t stream);
+
+// The kernel for few rows per KV head (kv8_attention.cuh; fp32: else 16-bit rows).
+template <int HD>
+cudaError_t launch_kv8_rows(const Kv8AttnParams& p, const Kv8Work& w, bool fp32, int32_t format,
+                            cudaStream_t stream);
 
 // The kernel for many rows per KV head (kv8_attention_tc.cu).
 bool kv8_tc_supported(int32_t dtype, int32_t head_dim);

@@ -68,7 +68,6 @@ constexpr int kConvRegs = 64;
 constexpr int kMmaRegs = 64;
 static_assert(2 * kSoftmaxRegs + 2 * kConvRegs + kMmaRegs <= 5 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
-constexpr int kSms = 148;
 constexpr float kMargin = 8.0f;
 
 template <int kFormat>
@@ -906,7 +905,7 @@ cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t
         if (e != cudaSuccess) return e;
         ready[dev] = true;
     }
-    return launch_programmatic(k, dim3(kSms), dim3(kThreads), Shape<HD>::SMEM, st, p, w);
+    return launch_programmatic(k, dim3(kKv8Sms), dim3(kThreads), Shape<HD>::SMEM, st, p, w);
 }
 
 template <typename T, int kFormat>
@@ -931,7 +930,7 @@ Kv8Work kv8_tc_work() {
     w.tile_rows = kRows;
     w.chunk = kKeys;
     w.min_run = 8;
-    w.target = kSms;
+    w.target = kKv8Sms;
     return w;
 }
 
