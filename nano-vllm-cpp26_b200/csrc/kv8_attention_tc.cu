@@ -739,31 +739,35 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                         }
                     }
                 };
-                // block ids two tiles ahead; a tile's exponents are used when the next
-                // tile's copies are on their way
-                Where w = find(item.c0), next = find(item.c0 + 1);
-                int e[2] = {0, 0};
-                uint32_t e_at = 0;
-                bool ok = true;
-                for (int t = 0; t < ntiles; ++t) {
+                auto check = [&](Where& x) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if (w.blk[i] != kNone && (w.blk[i] < 0 || w.blk[i] >= p.a.num_blocks)) {
+                        if (x.blk[i] != kNone && (x.blk[i] < 0 || x.blk[i] >= p.a.num_blocks)) {
                             atomicOr(p.status, kStatusBounds);
-                            w.blk[i] = kNone;
+                            x.blk[i] = kNone;
                         }
                     }
-                    ok = wait_all(&ctl->raw_free[kv][slot], slot_ph);
-                    if (!ok) break;
-                    int64_t off[2];
-                    int en[2];
+                };
+                auto load_exps = [&](const Where& x, int (&e)[2]) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        off[i] = w.blk[i] < 0 ? -1 : int64_t(w.blk[i]) * p.a.block_stride + int64_t(w.in[i]) * p.a.row;
-                        en[i] = -1000;
-                        if (w.blk[i] >= 0) {
-                            en[i] = __ldg(exps + int64_t(w.blk[i]) * p.a.exp_block_stride + exp_head + w.in[i]);
+                        e[i] = -1000;
+                        if (x.blk[i] >= 0) {
+                            e[i] = __ldg(exps + int64_t(x.blk[i]) * p.a.exp_block_stride + exp_head + x.in[i]);
                         }
+                    }
+                };
+                // block ids two tiles ahead, exponents one
+                Where x = find(item.c0), next = find(item.c0 + 1);
+                check(x);
+                int e[2];
+                load_exps(x, e);
+                for (int t = 0; t < ntiles; ++t) {
+                    if (!wait_all(&ctl->raw_free[kv][slot], slot_ph)) break;
+                    int64_t off[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        off[i] = x.blk[i] < 0 ? -1 : int64_t(x.blk[i]) * p.a.block_stride + int64_t(x.in[i]) * p.a.row;
                     }
                     const uint32_t dst = raw_addr + slot * S::RAW;
 #pragma unroll
@@ -776,15 +780,13 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
                                      smem_addr(&ctl->raw_full[kv][slot]))
                                  : "memory");
-                    w = next;
+                    write_factors(e, slot, n0 + t);
+                    x = next;
+                    check(x);
+                    load_exps(x, e);
                     next = find(item.c0 + t + 2);
-                    if (t > 0) write_factors(e, e_at, n0 + t - 1);
-                    e[0] = en[0];
-                    e[1] = en[1];
-                    e_at = slot;
                     if (++slot == kRaw) slot = 0, slot_ph ^= 1u;
                 }
-                if (ok) write_factors(e, e_at, n0 + ntiles - 1);
                 done(job);
             }
             kv8_copy_commit();
