@@ -184,7 +184,8 @@ enum nvllm_kv8_format {
  * Exponents: [num_blocks, num_layers, num_heads, block_size] int8 (the
  * positions of a block adjacent, as the attention reads them). num_heads of the
  * layout counts KV heads. A call reads no slot beyond a sequence's context, so
- * the arenas need no clearing. */
+ * the arenas need no clearing; what it does read must be what nvllm_kv8_write
+ * wrote (the two E4M3 codes that are not numbers never are). */
 typedef struct nvllm_kv8_arena {
     void* k_codes;
     void* v_codes;
@@ -230,12 +231,15 @@ size_t nvllm_kv8_attention_workspace_size(int32_t num_seqs, int32_t max_query_le
  * window > 0: the row at position p sees the positions j <= p with
  * j > p - window or j < sinks (a sliding window of `window` positions, itself
  * included, and the sequence's first `sinks` positions); window 0: all j <= p
- * (sinks is then not used). Positions whose block id lies outside the arena
+ * (sinks is then not used). Blocks of which no row sees a position may have been
+ * freed: their table entries are not read. Positions whose block id lies outside the arena
  * count as zero rows and raise NVLLM_ERR_BOUNDS; a sequence whose metadata
  * contradicts the maxima is skipped (its rows stay as they were) and raises
  * NVLLM_ERR_INVALID in nvllm_get_last_error. Rows that belong to no sequence
- * are not touched. The workspace (256-byte aligned) is overwritten by each
- * call: calls that may overlap on the GPU need one each. */
+ * are not touched. At most 65535 sequences. The workspace (256-byte aligned; one
+ * sized for larger maxima of the same layout and query heads serves) is
+ * overwritten by each call: calls that may overlap on the GPU need one each. A
+ * first call on a device belongs outside stream capture: it loads the kernels. */
 int nvllm_kv8_attention(void* out, int64_t out_stride, const void* query, int64_t query_stride,
                         int32_t dtype, const nvllm_kv8_arena* arena,
                         const int32_t* block_tables, int32_t max_blocks_per_seq,

@@ -124,6 +124,9 @@ constexpr int kv8_resident(int head_dim, int nq) { return head_dim * nq >= 512 |
 // Most sequences of a call without a plan (longer batches take several).
 constexpr int kKv8SelfSeqs = 512;
 
+// (The kernels start while the one before them drains, which may be writing the
+// cache: their loads are plain ones, never through the read-only path.)
+
 // Carves the workspace for a work list whose tile_rows, chunk, min_run and target
 // are set (base may be NULL to learn the size, returned in bytes).
 size_t kv8_work_layout(Kv8Work& w, unsigned char* base, int32_t num_seqs, int32_t max_query_len,

@@ -83,8 +83,8 @@ bool attention_sizes_ok(int32_t num_seqs, int32_t max_query_len, int32_t max_con
                         int32_t num_query_heads, const nvllm_kv_layout* lay) {
     return num_seqs >= 0 && max_query_len >= 1 && max_context_len >= max_query_len &&
            num_query_heads >= lay->num_heads && num_query_heads % lay->num_heads == 0 &&
-           // rows of a sequence, counted over the heads of a group, and the
-           // grid's (sequence, head) pairs stay within 32 bits
+           // rows of a sequence, counted over the heads of a group, and (sequence,
+           // head) pairs stay within 32 bits
            int64_t(max_query_len) * (num_query_heads / lay->num_heads) <= INT32_MAX / 2 &&
            int64_t(num_seqs) * num_query_heads <= INT32_MAX / 2 && num_seqs <= 65535;
 }
@@ -168,8 +168,10 @@ int nvllm_kv8_attention(void* out, int64_t out_stride, const void* query, int64_
     p.max_query_len = max_query_len;
     p.max_context_len = max_context_len;
     p.group = num_query_heads / layout->num_heads;
-    p.window = window;
-    p.sinks = window > 0 ? sinks : 0;
+    // a window that no context outgrows is none; so bounded, the kernels' sums of
+    // positions stay within 32 bits
+    p.window = window >= max_context_len ? 0 : window;
+    p.sinks = p.window > 0 ? (sinks < max_context_len ? sinks : max_context_len) : 0;
     p.qk_scale_log2 = scale * kLog2e;
     const cudaError_t e = launch_kv8_attention(p, dtype, arena->format, workspace,
                                                static_cast<cudaStream_t>(stream));

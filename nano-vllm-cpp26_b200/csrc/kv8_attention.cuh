@@ -397,8 +397,8 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             x.exps = 0;
             if (x.blk >= 0) {
                 const int8_t* e = lane < 16 ? p.a.k_exps : p.a.v_exps;
-                x.exps = __ldg(e + int64_t(x.blk) * p.a.exp_block_stride + int64_t(h) * p.a.block_size +
-                               (kB16 ? x.in + (lane & 15) : x.in));
+                x.exps = e[int64_t(x.blk) * p.a.exp_block_stride + int64_t(h) * p.a.block_size +
+                           (kB16 ? x.in + (lane & 15) : x.in)];
             }
             return x;
         };

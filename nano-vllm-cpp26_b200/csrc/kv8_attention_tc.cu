@@ -411,7 +411,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     raw[i] = make_uint4(0, 0, 0, 0);
-                    if (live) raw[i] = __ldg(src + i);
+                    if (live) raw[i] = src[i];
                     const T* v = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(to_float(v[k])));
@@ -697,7 +697,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                             (p.window <= 0 || pos > pos_lo - p.window || pos < p.sinks)) {
                             int entry;
                             kv8_place(p.a, pos, entry, x.in[i]);
-                            x.blk[i] = __ldg(table + entry);
+                            x.blk[i] = table[entry];
                         }
                     }
                     return x;
@@ -753,7 +753,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     for (int i = 0; i < 2; ++i) {
                         e[i] = -1000;
                         if (x.blk[i] >= 0) {
-                            e[i] = __ldg(exps + int64_t(x.blk[i]) * p.a.exp_block_stride + exp_head + x.in[i]);
+                            e[i] = exps[int64_t(x.blk[i]) * p.a.exp_block_stride + exp_head + x.in[i]];
                         }
                     }
                 };

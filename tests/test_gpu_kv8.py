@@ -273,6 +273,35 @@ def test_window_and_sinks(nv, torch, dtype, window, sinks, seqs, heads, kv, hd):
     b.check()
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("window", [513, 1 << 20, 2 ** 31 - 1])
+@pytest.mark.parametrize("seqs", [DECODES, CHUNKS], ids=["decodes", "chunks"])
+def test_windows_no_context_outgrows(nv, torch, dtype, window, seqs):
+    b = Batch(nv, torch, seqs, 2, 1, 128, dtype=dtype, window=window, sinks=2 ** 31 - 1, seed=9)
+    b.call()
+    b.check()
+
+
+def test_more_sequences_than_one_launch_counts(nv, torch):
+    """Over 512 decodes in one call, some without rows, ragged."""
+    seqs = [(1 if i % 5 else 0, 1 + (i * 37) % 90) for i in range(1100)] + [(1, 2000)]
+    b = Batch(nv, torch, seqs, 2, 1, 64, dtype="bf16", seed=4)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_one_workspace_serves_smaller_calls(nv, torch, dtype):
+    """Sized once for the largest step, used for all kinds after one another."""
+    ws = None
+    for seqs in ([(300, 900), (1, 2000), (5, 5)], [(1, 2000), (1, 700)], [(2, 2000)], [(9, 40), (1, 600)], [(64, 2000)], [(1, 1)]):
+        b = Batch(nv, torch, seqs, 4, 2, 128, dtype=dtype, seed=len(seqs))
+        if ws is None:
+            ws = nv.kv8_alloc_workspace(3, 300, 2000, 4, b.arena.layout)
+        b.call(workspace=ws)
+        b.check()
+
+
 @pytest.mark.parametrize("block", [1, 8, 16, 24, 32])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("seqs", [[(1, 700), (1, 90)], [(7, 400), (90, 600)]], ids=["decodes", "chunks"])

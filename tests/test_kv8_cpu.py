@@ -82,6 +82,17 @@ def test_workspace_sizes(nv):
     assert nv.kv8_workspace_size(1, 1, 1, 8, nv.KVLayout(4, 1, 16, 8, 96)) == 0
 
 
+@pytest.mark.parametrize("kv,heads,hd", [(1, 1, 64), (8, 32, 128), (32, 32, 128), (2, 32, 256), (4, 4, 32), (600, 600, 64)])
+def test_a_workspace_serves_every_smaller_call(nv, kv, heads, hd):
+    lay = nv.KVLayout(1 << 16, 1, 16, kv, hd)
+    sizes = [(s, q, c) for s in (1, 3, 64, 700) for q in (1, 2, 7, 33, 300, 4096) for c in (1, 300, 512, 513, 1280, 5000, 70000) if q <= c]
+    size = {k: nv.kv8_workspace_size(*k, heads, lay) for k in sizes}
+    for a in sizes:
+        for b in sizes:
+            if all(x <= y for x, y in zip(a, b)):
+                assert size[a] <= size[b], (a, b)
+
+
 def test_arena_checks_its_tensors(nv):
     import torch
     lay = nv.KVLayout(2, 1, 16, 2, 64)
