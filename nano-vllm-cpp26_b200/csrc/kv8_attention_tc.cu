@@ -35,6 +35,12 @@
 // 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
 // special function units, as many as the products take on the tensor cores at
 // head_dim 128.
+// Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.30
+// ms, 741 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 126 us. On the way:
+// one MMA warp for both halves 1.57 ms (its own instructions paced it), four
+// converter warps that also loaded 1.55, factors written a tile late 1.44. A step of
+// 128 keys with one S per half was slower, 1.69: S is then exposed behind the
+// softmax.
 // Every wait is bounded; on a timeout the CTA records NVLLM_ERR_TIMEOUT, lets its
 // MMAs finish and frees its TMEM.
 #include <algorithm>

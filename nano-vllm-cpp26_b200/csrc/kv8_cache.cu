@@ -14,7 +14,8 @@
 // KV head), the floor being that at the copy rate. In the write a thread owns 16
 // values of K and the same 16 of V (one 16-byte store of codes each), hd / 16
 // neighbouring lanes share a row and find its maximum by shuffles; all of a
-// thread's loads are in flight before the first is used.
+// thread's loads are in flight before the first is used. Measured on B200, 10229
+// tokens of 32 x 128 fp32: 70 us, 6.0 TB/s (0.92 of the copy rate).
 #include "kv8.cuh"
 
 namespace nvllm {
@@ -164,8 +165,8 @@ kv8_write_kernel(const Kv8Arena a, const Kv8Rows r) {
 
 // The read's pieces are 16 bytes of output (4 or 8 values), so that a warp's stores
 // are whole lines; a thread takes kReads of them, kThreads apart, of K and of V.
-// With the write's pieces (16 values, four strided 16-byte stores of fp32) the read
-// of 32768 rows of 32 x 128 took 288 us, 4.7 TB/s.
+// Measured on B200, 32768 rows of 32 x 128 to fp32: 262 us, 5.1 TB/s (four pieces a
+// thread 274; the write's pieces, four strided 16-byte stores of fp32, 288).
 constexpr int kReads = 2;
 
 template <typename T, int kFormat, bool kVec>
