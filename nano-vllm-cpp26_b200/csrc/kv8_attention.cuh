@@ -413,6 +413,8 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             int e[SUB];
         };
         const int64_t piece = int64_t(h) * HD + lane % R::PIECES * 16;
+        const int64_t lane_row = piece + lane / R::PIECES * p.a.row;  // kB16: of the lane's first row
+        const int64_t step_row = R::STEP * p.a.row;
         auto issue = [&](int c, int n, int b) -> Exps {
             Exps r;
             const int base = base_of(c);
@@ -423,16 +425,21 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const Where x = locate(c, n, u);
                 r.e[u] = x.exps;
                 const uint32_t dst = smem_addr(ring + b * S::BUF + u * 2 * R::TILE);
+                const int64_t tile = int64_t(x.blk) * p.a.block_stride + int64_t(x.in) * p.a.row + lane_row;
 #pragma unroll
                 for (int i = 0; i < R::COPIES; ++i) {
                     const int row = lane / R::PIECES + i * R::STEP;
-                    int blk = x.blk, in = x.in + row;
-                    if constexpr (!kB16) {
-                        blk = __shfl_sync(0xffffffffu, x.blk, row);
-                        in = __shfl_sync(0xffffffffu, x.in, row);
+                    int64_t at = tile + i * step_row;
+                    bool on = x.blk >= 0;
+                    if constexpr (kB16) {
+                        if (!all) on = on && seen(base + u * kSub + row);
+                    } else {
+                        const int blk = __shfl_sync(0xffffffffu, x.blk, row);
+                        const int in = __shfl_sync(0xffffffffu, x.in, row);
+                        on = blk >= 0;
+                        at = int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + piece;
                     }
-                    const bool on = blk >= 0 && (!kB16 || all || seen(base + u * kSub + row));
-                    const int64_t at = on ? int64_t(blk) * p.a.block_stride + int64_t(in) * p.a.row + piece : 0;
+                    at = on ? at : 0;
                     const uint32_t to = dst + R::at(row, lane % R::PIECES * 16);
                     kv8_copy16(to, p.a.k_codes + at, on);
                     kv8_copy16(to + R::TILE, p.a.v_codes + at, on);
