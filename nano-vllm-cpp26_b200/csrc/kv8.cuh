@@ -104,6 +104,7 @@ struct Kv8Work {
     int32_t chunk;
     int32_t min_run;   // shortest run (chunks) a tile is cut into
     int32_t target;    // runs to aim for, over all KV heads
+    int32_t round;     // items that run at once (0: not used)
     int32_t groups;    // > 0: one tile per sequence, cut into that many equal ranges (no plan)
     int32_t snap;      // ranges end where sequences do: no tile is cut
     int32_t merge_grid;  // CTAs of the merge, 0: no tile is ever cut

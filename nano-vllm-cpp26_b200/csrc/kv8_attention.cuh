@@ -37,8 +37,8 @@
 // joined through shared memory at the end of a run.
 //
 // Measured on B200: 64 sequences of 512-4096 positions, 32 heads x 128, fp32 rows:
-// 240 us, 5.1 TB/s (0.78 of the copy rate), 380 instructions per 16 positions at 47 %
-// issue with 12 warps an SM; 4 x 32768 positions, 32 heads over 8, bf16 rows: 84 us.
+// 230-245 us, up to 5.3 TB/s (0.81 of the copy rate), latency-bound at 47 % issue with
+// 12 warps an SM; 4 x 32768 positions, 32 heads over 8, bf16 rows: 82 us.
 // The order with query rows on the MMA's 16 rows took 518 us for the first, the
 // transposed one with fragments loaded straight into registers 280.
 #pragma once

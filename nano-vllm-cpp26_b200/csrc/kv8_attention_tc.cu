@@ -35,10 +35,11 @@
 // 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
 // special function units, as many as the products take on the tensor cores at
 // head_dim 128.
-// Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.30
-// ms, 741 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 126 us. On the way:
+// Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.19
+// ms, 812 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 126 us. On the way:
 // one MMA warp for both halves 1.57 ms (its own instructions paced it), four
-// converter warps that also loaded 1.55, factors written a tile late 1.44. A step of
+// converter warps that also loaded 1.55, factors written a tile late 1.44, no tile of
+// the last round cut 1.30. A step of
 // 128 keys with one S per half was slower, 1.69: S is then exposed behind the
 // softmax.
 // Every wait is bounded; on a timeout the CTA records NVLLM_ERR_TIMEOUT, lets its
@@ -939,6 +940,7 @@ Kv8Work kv8_tc_work() {
     w.chunk = kKeys;
     w.min_run = 8;
     w.target = kKv8Sms;
+    w.round = kKv8Sms;
     return w;
 }
 

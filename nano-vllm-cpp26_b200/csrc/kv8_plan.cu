@@ -6,6 +6,12 @@
 // as equal as they come, so that a few long sequences fill the GPU as well as many
 // short ones. A tile of n > L chunks has ceil(n / L) <= 2 n / L parts, so there are
 // at most 2 target partial slots over all heads, whatever the batch.
+//
+// Where no tile is that long (a late chunk of a long prompt: many tiles of nearly
+// one length) the tiles of the last, partly filled round of CTAs are cut instead, in
+// as many parts as fill it: 512 tiles of 192-256 key tiles on 148 CTAs take 3.5
+// rounds in place of 4. Tiles are counted in the order of the sequences, so that the
+// same ones are cut every time.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -22,6 +28,9 @@ size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
 template <bool kWide>
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnParams p, const Kv8Work w) {
     __shared__ unsigned long long total;
+    __shared__ int longest;
+    __shared__ int tiles_before[kWide ? kPlanThreads : 1];  // kWide: of earlier sequences
+    __shared__ int warp_tiles[kPlanThreads / 32];
     __shared__ int n_items, n_slots, n_merges;
     const int lane = threadIdx.x & 31;
     const int me = kWide ? threadIdx.x >> 5 : threadIdx.x;
@@ -30,22 +39,64 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
     const int t0 = kWide ? lane : 0;
     if (threadIdx.x == 0) {
         total = 0;
+        longest = 0;
         n_items = n_slots = n_merges = 0;
     }
     pdl_release();
     pdl_wait();  // the metadata may come from the kernel before; the workspace is its
     __syncthreads();
+    if constexpr (kWide) tiles_before[threadIdx.x] = 0;
+    __syncthreads();
     long long mine = 0;
+    int most = 0;
     for (int s = me; s < p.num_seqs; s += kSeqs) {
         const Kv8Seq q = kv8_seq(p, w, s);
         if (q.rows < 0 && t0 == 0) raise_status(kStatusMetadata);
-        for (int t = t0; t < q.ntiles; t += kStep) mine += kv8_list(p, w, q, t).n;
+        for (int t = t0; t < q.ntiles; t += kStep) {
+            const int n = kv8_list(p, w, q, t).n;
+            mine += n;
+            most = max(most, n);
+        }
+        if (kWide && lane == 0 && s < kPlanThreads) tiles_before[s] = q.ntiles;
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) atomicMax(&longest, most);
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0 && mine) atomicAdd(&total, (unsigned long long)mine);
     __syncthreads();
     const long long all = (long long)total * p.a.num_heads;
     const int run = int(max((long long)w.min_run, (all + w.target - 1) / w.target));
+    // from which tile on (in the order of the sequences) the last round's are cut
+    int cut_from = INT32_MAX, cut_parts = 1;
+    if constexpr (kWide) {
+        int x = tiles_before[threadIdx.x];
+        const int own = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_tiles[threadIdx.x >> 5] = x;
+        __syncthreads();
+        int tiles = 0;
+        x -= own;
+        for (int i = 0; i < kPlanThreads / 32; ++i) {
+            if (i < int(threadIdx.x >> 5)) x += warp_tiles[i];
+            tiles += warp_tiles[i];
+        }
+        tiles_before[threadIdx.x] = x;
+        __syncthreads();
+        const int H = p.a.num_heads;
+        const long long units = (long long)tiles * H;
+        const long long rest = w.round > 0 ? units % w.round : 0;
+        // lists of one length, or nearly (three quarters on average), and none cut
+        if (p.num_seqs <= kPlanThreads && units > w.round && rest > 0 && run >= longest &&
+            (long long)total * 4 >= (long long)longest * tiles * 3) {
+            const int last = int((rest + H - 1) / H);  // tiles of the last round
+            cut_parts = w.round / (last * H);
+            if (cut_parts > 1) cut_from = tiles - last;
+        }
+    }
     // the longest lists, those of a sequence's last tiles, go out first
     for (int base = 0; base < p.num_seqs; base += kSeqs) {
         const int s = base + me;
@@ -54,7 +105,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
             const int t = q.ntiles - 1 - i - t0;
             if (!__any_sync(0xffffffffu, t >= 0)) break;
             const Kv8List l = t >= 0 ? kv8_list(p, w, q, t) : Kv8List{0, 0, 0};
-            const int parts = t < 0 ? 0 : l.n > run ? (l.n + run - 1) / run : 1;
+            int parts = t < 0 ? 0 : l.n > run ? (l.n + run - 1) / run : 1;
+            if (kWide && t >= 0 && cut_from != INT32_MAX && tiles_before[s] + i + t0 >= cut_from) {
+                parts = max(1, min(cut_parts, l.n / (4 * w.min_run)));  // shorter ones cost what they save
+            }
             const int slots = parts > 1 ? parts : 0;
             // this lane's places: an inclusive scan of both counts in one word
             long long x = ((long long)(slots) << 32) | (unsigned)parts;

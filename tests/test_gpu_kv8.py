@@ -342,6 +342,27 @@ def test_long_contexts_are_split_and_joined(nv, torch, dtype, seqs):
     b.check()
 
 
+@pytest.mark.parametrize("seqs", [[(1024, 5000)], [(300, 4900), (700, 5000)]], ids=["one", "two"])
+def test_the_last_round_of_tiles_is_cut(nv, torch, seqs):
+    """A few more tiles of nearly one length than CTAs: the last ones are shared out
+    and merged, the same way every time."""
+    heads = 40
+    b = Batch(nv, torch, seqs, heads, heads, 64, dtype="bf16", seed=21)
+    b.call()
+    first = b.out.clone()
+    b.out.fill_(9.0)
+    b.call()
+    assert torch.equal(first, b.out)
+    q = values64(b.query).reshape(-1, heads, 64)
+    out = values64(b.out).reshape(-1, heads, 64)
+    some = [0, 39]
+    at = 0
+    for s, (new, ctx) in enumerate(seqs):
+        want, sizes = ref.attention(q[at : at + new, some], b.k[s][:, some], b.v[s][:, some], ctx - new, 1, 0.125)
+        assert (np.abs(out[at : at + new, some] - want) <= ref.tolerance(want, sizes, 64, "bf16")).all()
+        at += new
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("seqs", [DECODES, CHUNKS], ids=["decodes", "chunks"])
 def test_wide_magnitudes(nv, torch, dtype, seqs):
