@@ -910,6 +910,12 @@ cudaError_t launch_kernel(const Kv8AttnParams& p, const Kv8Work& w, cudaStream_t
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!ready[dev]) {
+        // the split counts on what the block is launched with: with fewer registers
+        // the softmax warps would wait for theirs for good
+        cudaFuncAttributes attr{};
+        e = cudaFuncGetAttributes(&attr, k);
+        if (e != cudaSuccess) return e;
+        if (attr.numRegs < kLaunchRegs) return cudaErrorInvalidConfiguration;
         e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<HD>::SMEM));
         if (e != cudaSuccess) return e;
         ready[dev] = true;
