@@ -32,16 +32,20 @@
 //                   exponents; rows that no query of the tile sees are 0.
 // The last three warpgroups give registers to the softmax.
 // TMEM (512 columns): S of half i, buffer b at 128 i + 64 b, O of half i at 256 +
-// 128 i. The exponentials bound it: 64 x 256 per key tile are 1024 cycles of the
-// special function units, as many as the products take on the tensor cores at
-// head_dim 128.
+// 128 i.
+//
+// A key tile costs at least 1024 cycles of the special function units (64 x 256
+// exponentials) and, at head_dim 128, as many of the tensor cores. It takes about
+// 2400: MMAs on different accumulators have no order of their own, so the S that
+// takes P's place waits until O is complete, and an S of N = 64 is paced by Q's
+// re-reads from shared memory (66 cycles in place of 32).
 // Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.19
-// ms, 812 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 126 us. On the way:
+// ms, 812 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 128 us. On the way:
 // one MMA warp for both halves 1.57 ms (its own instructions paced it), four
-// converter warps that also loaded 1.55, factors written a tile late 1.44, no tile of
-// the last round cut 1.30. A step of
-// 128 keys with one S per half was slower, 1.69: S is then exposed behind the
-// softmax.
+// converter warps that also loaded 1.55, factors written a tile late 1.44, no tile
+// of the last round cut 1.30. A step of 128 keys with one S per half was slower, 1.69
+// against 1.44: S is then exposed behind the softmax.
+//
 // Every wait is bounded; on a timeout the CTA records NVLLM_ERR_TIMEOUT, lets its
 // MMAs finish and frees its TMEM.
 #include <algorithm>
