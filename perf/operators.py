@@ -259,19 +259,14 @@ def _plain(s):
     return {"key": s["key"], "value": s["value"]}
 
 
-_package = None
-
-
 def _nvllm():
-    """The framework, imported once as a program does."""
-    global _package
-    if _package is None:
-        import sys
-        from pathlib import Path
-        sys.path.insert(0, str(Path.cwd() / "nano-vllm-cpp26_b200"))
-        import nvllm
-        _package = nvllm
-    return _package
+    import sys
+    from pathlib import Path
+    package = str(Path.cwd() / "nano-vllm-cpp26_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import nvllm
+    return nvllm
 
 
 def _own(s):
