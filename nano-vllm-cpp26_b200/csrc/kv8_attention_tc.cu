@@ -108,7 +108,7 @@ struct Control {
     uint64_t drain[2];
     uint64_t item_full[2];      // two-slot queue of work items
     uint64_t item_free[2];
-    uint64_t q_full[2];         // Q of a half of the item written
+    uint64_t q_full[2];         // Q of a half written, items with rows in the half counted
     int32_t top[kTops];         // A of a key tile
     int32_t large[kRaw];        // some V exponent of a key tile is above 7
     uint32_t tmem_base;
@@ -442,8 +442,8 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     *reinterpret_cast<uint4*>(dst + (i >> 3) * S::Q_ATOM + ((i & 7) ^ (r & 7)) * 16) = o;
                 }
                 tc::fence_async_smem();
+                warp_arrive(&ctl->q_full[half]);
             }
-            warp_arrive(&ctl->q_full[half]);
             const int pos = first_pos + (item.row0 + min(half * kHalf + r, nrows - 1)) / p.group;
             float m = -INFINITY, l = 0.f;
             bool ok = true;
@@ -821,15 +821,22 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
             };
             uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;  // stage and phase of the next S and O
             uint32_t s_n = 0, o_n = 0;                        // S and O of this half so far
+            uint32_t q_n = 0;                                 // items with rows in this half so far
             for (uint32_t j = 0;; ++j) {
                 const int it = next_item(j);
                 if (it < 0) break;
                 const Job job = job_of(it);
                 const int ntiles = int(uniform(uint32_t(job.ntiles)));
                 const bool on = uniform(uint32_t(job.halves)) > i;
+                // q_full counts only items with rows in this half, on both sides: over the
+                // others this warp and the half's softmax each run ahead of the other by up
+                // to two items, and a phase per item would be mistaken for another's. The
+                // softmax cannot leave an item of its half without this warp's S, so neither
+                // is ever a counted phase ahead.
+                bool ok = !on || wait_all(&ctl->q_full[i], q_n & 1u);
+                q_n += on;
                 // t < 0: the first two S. Then O(t) and the S that takes its P's place; the
                 // softmax works on S(t + 1) meanwhile.
-                bool ok = !on || wait_all(&ctl->q_full[i], j & 1u);
                 for (int t = -2; ok && t < ntiles; ++t) {
                     if (t >= 0) {
                         const uint32_t b = o_n & 1u;
