@@ -13,6 +13,7 @@ that device's current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -150,6 +151,15 @@ def _call(arena: KV8Arena, stream, f, *args) -> int:
         return f(*args, stream)
 
 
+def _stream_scope(stream, device):
+    """A context in which ``stream`` (None, a raw handle or a Stream) is current."""
+    import torch
+    if isinstance(stream, int):
+        stream = (torch.cuda.ExternalStream(stream, device=device) if stream > 1  # (0, 1: legacy)
+                  else torch.cuda.default_stream(device))
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
 def _move(what: str, f, key, value, arena: KV8Arena, slot_mapping, layer: int, stream,
           check: bool) -> int:
     width = arena.layout.hidden
@@ -207,7 +217,8 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
     ``query`` and ``out`` [rows, num_heads * head_dim] (``num_heads`` query heads, a
     multiple of the layout's KV heads; default: as many). Metadata as in
     :func:`nvllm.paged_attention`. ``window`` > 0 keeps, for the row at position
-    p, the positions above p - window and the first ``sinks`` ones."""
+    p, the positions above p - window and the first ``sinks`` ones. Without a
+    ``workspace`` the call allocates one on its stream."""
     layout = arena.layout
     if num_heads is None:
         num_heads = layout.num_heads
@@ -226,10 +237,10 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
     if scale is None:
         scale = 1.0 / math.sqrt(layout.head_dim)
     if workspace is None:
-        workspace = kv8_alloc_workspace(num_seqs, max_query_len, max_context_len, num_heads, layout,
-                                        arena.device)
-        if stream is not None and not isinstance(stream, int):
-            workspace.record_stream(stream)  # it is freed here, in use there
+        # on the call's stream: the allocator orders a block's uses on the stream it came from
+        with _stream_scope(stream, arena.device):
+            workspace = kv8_alloc_workspace(num_seqs, max_query_len, max_context_len, num_heads, layout,
+                                            arena.device)
     elif workspace.get_device() != arena.index:
         raise ValueError(f"workspace must be on the arena's device {arena.device}")
     st = _call(arena, stream, _lib().nvllm_kv8_attention, out.data_ptr(), _stride(out),

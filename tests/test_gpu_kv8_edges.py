@@ -32,3 +32,33 @@ def test_full_and_half_tiles_in_turn(nv, torch, dtype, hd):
         b.out.fill_(9.0)
         b.call()
         assert torch.equal(first, b.out)
+
+
+@pytest.mark.parametrize("raw", [False, True], ids=["stream", "handle"])
+def test_default_workspaces_on_two_streams(nv, torch, raw):
+    """Calls without a workspace on a side stream, while the current stream keeps
+    allocating, filling and freeing tensors of the workspace's size."""
+    seqs = [(1, 2500), (1, 900), (1, 1700), (1, 40)]
+    b = Batch(nv, torch, seqs, 8, 2, 128, dtype="bf16", seed=31)
+    size = nv.kv8_workspace_size(len(seqs), b.max_new, b.max_ctx, 8, b.arena.layout)
+    st = torch.cuda.Stream()
+    outs = [torch.full_like(b.out, 9.0) for _ in range(40)]
+    st.wait_stream(torch.cuda.current_stream())
+    for out in outs:
+        junk = torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255)
+        b.call(out=out, stream=st.cuda_stream if raw else st)
+        del junk
+        junk = torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255)
+        del junk
+    torch.cuda.synchronize()
+    b.check(outs[0])
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("handle", [0, None], ids=["legacy", "current"])
+def test_default_workspace_on_the_default_streams(nv, torch, handle):
+    b = Batch(nv, torch, [(1, 2500), (3, 40)], 4, 2, 64, seed=32)
+    torch.cuda.synchronize()
+    b.call(stream=handle)
+    torch.cuda.synchronize()
+    b.check()

@@ -1,0 +1,127 @@
+"""The Python binding of the 8-bit cache without a GPU: which stream and device a
+call and its default workspace are on, with stand-ins for tensors and torch.cuda."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+
+
+class Tensor:
+    """What the binding asks of a CUDA tensor."""
+
+    def __init__(self, *shape, dtype, device=0, stride=None, contiguous=True, size=None):
+        self.shape, self.dtype, self.device, self.contiguous = shape, dtype, device, contiguous
+        self.strides = stride or (shape[-1], 1)[-len(shape):]
+        self.size = size if size is not None else 4
+
+    def get_device(self):
+        return self.device
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i):
+        return self.strides[i]
+
+    def numel(self):
+        n = 1
+        for s in self.shape:
+            n *= s
+        return n
+
+    def element_size(self):
+        return self.size
+
+    def is_contiguous(self):
+        return self.contiguous
+
+    def data_ptr(self):
+        return 4096
+
+    def record_stream(self, stream):
+        pass
+
+
+class World:
+    """torch.cuda as the binding sees it, and the calls that reach the library."""
+
+    def __init__(self, monkeypatch, nv):
+        import torch
+        from nvllm import kv8
+        self.current, self.device, self.allocated, self.calls = 1000, 0, [], []
+        self.kv8, self.torch, self.layout = kv8, torch, nv.KVLayout(8, 1, 16, 2, 64)
+
+        def library(name):
+            def f(*args):
+                self.calls.append(SimpleNamespace(name=name, args=args, stream=args[-1], device=self.device))
+                return 0
+            return f
+
+        @contextlib.contextmanager
+        def use(stream):
+            before, self.current = self.current, stream.cuda_stream
+            yield
+            self.current = before
+
+        @contextlib.contextmanager
+        def on(index):
+            before, self.device = self.device, index
+            yield
+            self.device = before
+
+        def alloc(*args, **kw):
+            self.allocated.append(self.current)
+            return Tensor(1 << 20, dtype=torch.uint8, size=1, device=args[-1] if isinstance(args[-1], int) else 0)
+
+        def external(handle, device=None):
+            return SimpleNamespace(cuda_stream=handle)
+        names = ("nvllm_kv8_attention", "nvllm_kv8_write", "nvllm_kv8_read")
+        lib = SimpleNamespace(**{n: library(n) for n in names})
+        monkeypatch.setattr(kv8, "_lib", lambda: lib)
+        monkeypatch.setattr(kv8, "_DTYPES", {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        monkeypatch.setattr(kv8, "_INT32", torch.int32)
+        monkeypatch.setattr(kv8, "_RAW_STREAM", lambda index: self.current + index)
+        monkeypatch.setattr(kv8, "_CURRENT_DEVICE", lambda: self.device)
+        monkeypatch.setattr(kv8, "kv8_alloc_workspace", alloc)
+        monkeypatch.setattr(torch.cuda, "stream", use)
+        monkeypatch.setattr(torch.cuda, "device", on)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", external)
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: SimpleNamespace(cuda_stream=0))
+
+    def arena(self, index=0):
+        return SimpleNamespace(layout=self.layout, index=index, device=index, _ref=None, _lay=None)
+
+    def attention(self, index=0, rows=3, **kw):
+        t = self.torch
+        x = dict(device=index)
+        q, out = (kw.pop(n, Tensor(rows, 128, dtype=t.bfloat16, size=2, **x)) for n in ("query", "out"))
+        return self.kv8.kv8_attention(
+            out, q, self.arena(index), Tensor(2, 4, dtype=t.int32, **x), Tensor(3, dtype=t.int32, **x),
+            Tensor(2, dtype=t.int32, **x), kw.pop("max_query_len", 2), kw.pop("max_context_len", 20), kw.pop("layer", 0), **kw)
+
+
+@pytest.fixture
+def world(monkeypatch, nv):
+    return World(monkeypatch, nv)
+
+
+def test_default_workspace_is_allocated_on_the_calls_stream(world):
+    """The allocator orders a block's reuse on the stream that it was allocated on."""
+    for stream, handle in ((None, 1000), (2048, 2048), (SimpleNamespace(cuda_stream=4096), 4096), (0, 0)):
+        world.attention(stream=stream)
+        assert world.calls[-1].stream == handle
+        assert world.allocated[-1] == handle
+    assert world.current == 1000
+
+
+def test_calls_run_on_their_tensors_device(world):
+    t = world.torch
+    world.attention(index=1)
+    assert (world.calls[-1].device, world.calls[-1].stream) == (1, 1001)
+    rows = Tensor(2, 128, dtype=t.float32, device=1)
+    for f in (world.kv8.kv8_write, world.kv8.kv8_read):
+        f(rows, rows, world.arena(1), Tensor(2, dtype=t.int32, device=1), 0)
+        assert (world.calls[-1].device, world.calls[-1].stream) == (1, 1001)
+    assert world.device == 0
+    with pytest.raises(ValueError, match="device"):
+        world.kv8.kv8_write(rows, rows, world.arena(0), Tensor(2, dtype=t.int32, device=1), 0)
