@@ -14,7 +14,8 @@
 // codes become 16-bit floats, K's against the tile's largest, which is one more
 // factor of the row's scale. V is exact in bf16 whatever its exponent; K' in fp16
 // is exact for rows within 2^22 of the tile's largest (2^29 for INT8) and beyond
-// that off by 2^-36 of the largest. P is rounded to bf16, half a step of which is
+// that off by 2^-36 of the largest: a factor below fp16's range is taken in two
+// steps, of which only the last rounds. P is rounded to bf16, half a step of which is
 // the output's own; for fp16 rows, whose step is finer, P is two bf16 terms.
 //
 // One CTA per SM, 20 warps in 5 warpgroups:
@@ -110,6 +111,7 @@ struct Control {
     uint64_t item_free[2];
     uint64_t q_full[2];         // Q of a half written, items with rows in the half counted
     int32_t top[kTops];         // A of a key tile
+    int32_t small[kRaw];        // some K factor of a key tile is below fp16's range
     int32_t large[kRaw];        // some V exponent of a key tile is above 7
     uint32_t tmem_base;
     int32_t items[2];
@@ -206,7 +208,10 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t h) {
     return pack_bf16(a - f.x, b - f.y);
 }
 
-// 2^e as an fp16 pair, e <= 15 (below 2^-24: 0).
+// 2^e as an fp16 pair, e <= 15 (below 2^-24, the smallest fp16: 0).
+constexpr int kHalfMinExp = -24;
+// Any code times 2^-15 is an exact fp16: a multiple of 2^-24.
+constexpr int kCodeShift = 15;
 __device__ __forceinline__ __half2 half_power(int e) {
     return __float2half2_rn(exp2_int(max(e, -30)));
 }
@@ -610,6 +615,11 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     x[i] = *reinterpret_cast<const uint4*>(my_raw + slot * S::RAW + i * S::STEP * HD);
                     f[i].x = sFactor[(slot * kKeys + row0 + S::STEP * i) * 2];
                 }
+                const bool small = ctl->small[slot];
+                if (small) {
+#pragma unroll
+                    for (int i = 0; i < S::COPIES; ++i) f[i].y = sFactor[(slot * kKeys + row0 + S::STEP * i) * 2 + 1];
+                }
                 warp_arrive(&ctl->raw_free[0][slot]);
                 // a stage's first use waits for nothing (the phase before the first)
                 ok = wait_all(&ctl->k_free[st], st_ph);
@@ -618,11 +628,20 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                 for (int i = 0; i < S::COPIES; ++i) {
                     const __half2 f2 = *reinterpret_cast<const __half2*>(&f[i].x);
-                    uint4 a, b;
-                    scaled_half4<kFormat>(x[i].x, f2, a.x, a.y);
-                    scaled_half4<kFormat>(x[i].y, f2, a.z, a.w);
-                    scaled_half4<kFormat>(x[i].z, f2, b.x, b.y);
-                    scaled_half4<kFormat>(x[i].w, f2, b.z, b.w);
+                    uint32_t o[8];
+                    scaled_half4<kFormat>(x[i].x, f2, o[0], o[1]);
+                    scaled_half4<kFormat>(x[i].y, f2, o[2], o[3]);
+                    scaled_half4<kFormat>(x[i].z, f2, o[4], o[5]);
+                    scaled_half4<kFormat>(x[i].w, f2, o[6], o[7]);
+                    if (small) {
+                        const __half2 g = *reinterpret_cast<const __half2*>(&f[i].y);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&o[k]), g);
+                            o[k] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                    }
+                    const uint4 a = make_uint4(o[0], o[1], o[2], o[3]), b = make_uint4(o[4], o[5], o[6], o[7]);
                     *reinterpret_cast<uint4*>(stage + put0 + i * S::STEP * 128) = swap ? b : a;
                     *reinterpret_cast<uint4*>(stage + put1 + i * S::STEP * 128) = swap ? a : b;
                 }
@@ -715,19 +734,26 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 };
                 // The factors of the lane's two positions, from their exponents (-1000:
                 // nothing there): K's against the tile's largest, V's its own, in E4M3 with
-                // the 2^120 that the codes lack. That leaves bf16's range above 2^7: the
-                // rest is a second factor, which almost no tile has.
+                // the 2^120 that the codes lack. K's leaves fp16's range 2^31 below the
+                // largest (2^29 for INT8), V's bf16's above 2^7: the rest is a second
+                // factor, which almost no tile has.
                 auto write_factors = [&](const int (&e)[2], uint32_t at, uint32_t n) {
                     uint32_t* dst = factor + (at * kKeys + lane) * 2;
                     if (kv == 0) {
                         const int A = max(__reduce_max_sync(0xffffffffu, max(e[0], e[1])), kKv8MinExp);
+                        const int lowest = U - A + min(e[0] < kKv8MinExp ? A : e[0], e[1] < kKv8MinExp ? A : e[1]);
+                        const bool small = __any_sync(0xffffffffu, lowest < kHalfMinExp);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const __half2 f = half_power(e[i] - A + U);
+                            const int g = e[i] - A + U;
+                            const __half2 f = half_power(small ? max(g, -kCodeShift) : g);
+                            const __half2 rest = half_power(min(g + kCodeShift, 0));
                             dst[64 * i] = *reinterpret_cast<const uint32_t*>(&f);
+                            dst[64 * i + 1] = *reinterpret_cast<const uint32_t*>(&rest);
                         }
                         __syncwarp();
                         if (lane == 0) {
+                            ctl->small[at] = small;
                             ctl->top[n % kTops] = A;
                             mbar_arrive(&ctl->top_full[n % kTops]);
                             mbar_arrive(&ctl->raw_full[0][at]);

@@ -5,6 +5,7 @@ answer and the derived tolerance are those of test_gpu_kv8 and kv8_ref."""
 import numpy as np
 import pytest
 
+import kv8_ref as ref
 from test_gpu_kv8 import Batch, clean_status, dtype_of, fmt_id, torch, values64  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,26 @@ def test_default_workspace_on_the_default_streams(nv, torch, handle):
     b.call(stream=handle)
     torch.cuda.synchronize()
     b.check()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype,hd", [("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("by", [20, 28, 30, 32, 34])
+def test_keys_far_below_a_later_one(nv, torch, fmt, dtype, hd, by):
+    """The last key of a prompt is 2^by larger than the others of its 64: the rows
+    before it, which do not see it, are answered as if it were not there."""
+    seqs = [(40, 60), (1, 7), (70, 130)]
+    b = Batch(nv, torch, seqs, 8, 2, hd, fmt=fmt, dtype=dtype, seed=by)
+    for s, (_, ctx) in enumerate(seqs):
+        blk = int(b.tables[s, (ctx - 1) // 16])
+        b.arena.k_exp[blk, b.layer, :, (ctx - 1) % 16] += by
+        b.k[s][ctx - 1] *= 2.0 ** by
+    b.call()
+    out, q = (values64(x).reshape(-1, 8, hd) for x in (b.out, b.query))
+    at = 0
+    for s, (new, ctx) in enumerate(seqs):
+        rows = slice(at, at + new - 1)
+        at += new
+        if new > 1:
+            want, sizes = ref.attention(q[rows], b.k[s], b.v[s], ctx - new, 4, hd ** -0.5)
+            assert (np.abs(out[rows] - want) <= ref.tolerance(want, sizes, hd, dtype)).all()
