@@ -9,8 +9,14 @@
 //   P_j = 2^(x_j + b_j - m),  acc = sum_j P_j d_j,  l = sum_j 2^(x_j - m),  o = acc / l
 // Codes are exact in fp16, so the exponents never touch the products, and with m
 // the size of contributions (not of weights) P is in [0, 1] and the largest one
-// keeps all its bits however far apart the rows' exponents are; 2^(x_j - m) <=
-// 2^100 since b_j >= -100.
+// keeps all its bits however far apart the rows' exponents are.
+// Weights then lie between 2^-119 and 2^100 where they count (b_j is in [-100,
+// 119]), which leaves no room below for the small ones: with v_j = b_j - 23 in
+// place of b_j above, m is 23 lower, the exponential gives 2^(x_j - m) 2^23, and its
+// sum is taken times 2^-23 in the same instruction, so that nothing above 2^-149 is
+// lost. When m moves by more than fp32 spans, l must keep what P and acc may drop
+// (rows of zeros have b_j = -100 and may have all of the weight): l is rescaled by
+// the square root of the factor, twice.
 //
 // Operands are fp16 terms: q' of fp32 rows as two (2^-23 of the row's largest
 // element), of bf16 and fp16 rows as one (exact up to 2^-25 of the largest); P of
@@ -133,6 +139,16 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// The same down to 2^-149.
+__device__ __forceinline__ float ex2_full(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The weights' shift: 2^23 times a weight is at most 2^(100 + kMargin + 23) < 2^128.
+constexpr float kUpBy = 23.0f;
 
 // a, b as fp16 in one word (a low).
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
@@ -447,10 +463,10 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             }
             return r;
         };
-        auto store_exps = [&](const Exps& x, int b) {  // 2^a_j of the 16 positions, then b_j
+        auto store_exps = [&](const Exps& x, int b) {  // 2^a_j of the 16 positions, then b_j - kUpBy
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
-                sE[(b * SUB + u) * 32 + lane] = lane < 16 ? exp2_int(min(max(x.e[u], -126), 127)) : float(x.e[u]);
+                sE[(b * SUB + u) * 32 + lane] = lane < 16 ? exp2_int(min(max(x.e[u], -126), 127)) : float(x.e[u]) - kUpBy;
             }
         };
         Exps ahead{};
@@ -613,7 +629,8 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
                     const float mn = top > m[nq][i] + kMargin ? top : m[nq][i];
                     const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-                    alpha[nq][i] = ex2(m[nq][i] - mu);
+                    const float root = ex2_full(0.5f * (m[nq][i] - mu));
+                    alpha[nq][i] = root * root;
                     m[nq][i] = mn;
                     float sum = 0.f;
 #pragma unroll
@@ -621,10 +638,10 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const float y = x[u][k] - mu;
-                            sum += ex2(y);
+                            sum = fmaf(ex2(y), 0x1p-23f, sum);
                             pw[u][k][i] = ex2(y + vb[u][k]);
                         }
-                    l[nq][i] = fmaf(l[nq][i], alpha[nq][i], sum);
+                    l[nq][i] = fmaf(l[nq][i] * root, root, sum);
                 }
 #pragma unroll
                 for (int u = 0; u < SUB; ++u)
@@ -749,8 +766,9 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             float L = 0.f, f[kWarps];
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) {
-                f[k] = ex2(ml[k].x - mu);
-                L = fmaf(ml[k].y, f[k], L);
+                const float root = ex2_full(0.5f * (ml[k].x - mu));
+                f[k] = root * root;
+                L = fmaf(ml[k].y * root, root, L);
             }
             const int row = item.row0 + r;
             const int64_t slot = (int64_t(item.slot) * H + h) * S::ROWS + r;

@@ -213,8 +213,11 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p, c
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float f = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - M);
-                L = fmaf(ml[u].y, f, L);
+                // (a part may have all of the weight and 2^-200 of the values: the square
+                // root of the factor, twice)
+                const float root = ml[u].x == -INFINITY ? 0.f : exp2f(0.5f * (ml[u].x - M));
+                L = fmaf(ml[u].y * root, root, L);
+                const float f = root * root;
 #pragma unroll
                 for (int d = 0; d < PER; ++d) o[d] = fmaf(a[u][d], f, o[d]);
             }

@@ -86,3 +86,63 @@ def test_keys_far_below_a_later_one(nv, torch, fmt, dtype, hd, by):
         if new > 1:
             want, sizes = ref.attention(q[rows], b.k[s], b.v[s], ctx - new, 4, hd ** -0.5)
             assert (np.abs(out[rows] - want) <= ref.tolerance(want, sizes, hd, dtype)).all()
+
+
+class Rows:
+    """One sequence whose K and V are given: written by kv8_write, read back for the
+    64-bit answer."""
+
+    def __init__(self, nv, torch, q, k, v, dtype, fmt="e4m3", group=1, block=16):
+        ctx, kv, hd = k.shape
+        self.nv, self.torch, self.dtype, self.group = nv, torch, dtype, group
+        lay = nv.KVLayout(-(-ctx // block), 1, block, kv, hd)
+        self.arena = nv.KV8Arena.alloc(lay, fmt_id(nv, fmt))
+        slots = torch.arange(ctx, dtype=torch.int32, device="cuda")
+        rows = [torch.from_numpy(x.astype(np.float32)).cuda().reshape(ctx, kv * hd) for x in (k, v)]
+        nv.kv8_write(*rows, self.arena, slots, 0)
+        back = [torch.empty_like(x) for x in rows]
+        nv.kv8_read(*back, self.arena, slots, 0)
+        self.k, self.v = (values64(x).reshape(k.shape) for x in back)
+        self.q = torch.from_numpy(q.astype(np.float32)).cuda().reshape(len(q), -1).to(dtype_of(torch, dtype))
+        self.out = torch.full_like(self.q, 9.0)
+        ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (range(-(-ctx // block)), [0, len(q)], [ctx])]
+        nv.kv8_attention(self.out, self.q, self.arena, ints[0][None].contiguous(), ints[1], ints[2], len(q), ctx, 0,
+                         num_heads=kv * group)
+
+    def check(self):
+        n, (ctx, kv, hd) = len(self.q), self.k.shape
+        heads = kv * self.group
+        want, sizes = ref.attention(values64(self.q).reshape(n, heads, hd), self.k, self.v, ctx - n, self.group, 1 / np.sqrt(hd))
+        off = np.abs(values64(self.out).reshape(n, heads, hd) - want)
+        tol = ref.tolerance(want, sizes, hd, self.dtype)
+        assert np.isfinite(off).all() and (off <= tol).all(), float((off / tol).max())
+
+
+def normal(seed, *shape):
+    return np.random.default_rng(seed).standard_normal(shape)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,ctx", [(1, 300), (1, 5000), (60, 300)], ids=["one", "long", "chunk"])
+@pytest.mark.parametrize("power", [-90, 60, 112, 124])
+def test_values_at_the_ends_of_the_range(nv, torch, dtype, rows, ctx, power):
+    """Value rows of 2^power and so exponents of that size: small weights still count."""
+    if power == 124 and rows > 1 and dtype != "fp32":
+        pytest.skip("sums of 300 such values are beyond 32 bits")
+    Rows(nv, torch, normal(1, rows, 4, 64) * 1.5, normal(2, ctx, 2, 64), normal(3, ctx, 2, 64) * 2.0 ** power, dtype, group=2).check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,ctx", [(1, 100), (1, 400), (1, 6000), (60, 400)], ids=["short", "one", "long", "chunk"])
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("power", [30, 60, 100])
+def test_rows_of_zeros_beside_large_values(nv, torch, dtype, rows, ctx, first, power):
+    """Half the positions hold value rows of zeros, with nearly all of the weight; the
+    other half's values are about 2^power."""
+    q, k, v = (np.zeros((n, 1, 64)) for n in (rows, ctx, ctx))
+    q[:, :, 0], q[:, :, 1:] = 8.0, normal(4, rows, 1, 63) * 0.1
+    k[:, :, 1:] = normal(5, ctx, 1, 63)
+    heavy = (np.arange(ctx) < ctx // 2) == first
+    k[:, 0, 0] = np.where(heavy, 8.0, 0.0)              # a score of 8 more
+    v[~heavy] = normal(6, int((~heavy).sum()), 1, 64) * 2.0 ** power
+    Rows(nv, torch, q, k, v, dtype).check()
