@@ -8,7 +8,7 @@
 // of a key tile (U = 7 for E4M3, 5 for INT8):
 //   K'_j = c_j 2^(a_j - A + U)                 in fp16
 //   S = q' . K'_j,  x_j = S 2^(A - U) qs       log2-domain score
-//   m = running max of x_j,  P_j = 2^(x_j - m)   in bf16
+//   m = running max of x_j,  P_j = 2^(x_j - m - 16)   in bf16
 //   acc += sum_j P_j V_j,  l += sum_j P_j,  o = acc / l     V_j = d_j 2^(b_j) in bf16
 // The exponents cost nothing per score: they are folded into the operands while
 // codes become 16-bit floats, K's against the tile's largest, which is one more
@@ -81,6 +81,10 @@ constexpr int kMmaRegs = 64;
 static_assert(2 * kSoftmaxRegs + 2 * kConvRegs + kMmaRegs <= 5 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kMargin = 8.0f;
+// Weights are taken this much lower (log2; it cancels in acc / l): a weight can reach
+// 2^kMargin, a value 2^127.8, and their sums have to stay within fp32. bf16 has the
+// range, and 2^-16 of the smallest value, 2^-109, is a normal number still.
+constexpr float kDownBy = 16.0f;
 
 template <int kFormat>
 constexpr int kUp = kFormat == NVLLM_KV8_E4M3 ? 7 : 5;
@@ -515,7 +519,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     }
                 }
                 float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                const float2 f2 = make_float2(f, f), mu2 = make_float2(-mu, -mu);
+                const float2 f2 = make_float2(f, f), mu2 = make_float2(-mu - kDownBy, -mu - kDownBy);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     uint32_t pk[16], rest[16];

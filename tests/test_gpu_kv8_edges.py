@@ -146,3 +146,14 @@ def test_rows_of_zeros_beside_large_values(nv, torch, dtype, rows, ctx, first, p
     k[:, 0, 0] = np.where(heavy, 8.0, 0.0)              # a score of 8 more
     v[~heavy] = normal(6, int((~heavy).sum()), 1, 64) * 2.0 ** power
     Rows(nv, torch, q, k, v, dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_large_values_whose_scores_grow_slowly(nv, torch, dtype, rows):
+    """Scores that rise by less than the step at which a kernel moves its reference,
+    with values near the end of the range."""
+    ctx = 700
+    q, k = np.zeros((rows, 1, 64)), np.zeros((ctx, 1, 64))
+    q[:, :, 0], k[64:, :, 0] = 1.0, 8 * 7.5 * np.log(2.0)  # 2^7.5 times the weight of the first 64
+    Rows(nv, torch, q, k, np.abs(normal(7, ctx, 1, 64)) * 2.0 ** 116, dtype).check()
