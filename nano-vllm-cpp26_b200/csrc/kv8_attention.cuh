@@ -10,13 +10,13 @@
 // Codes are exact in fp16, so the exponents never touch the products, and with m
 // the size of contributions (not of weights) P is in [0, 1] and the largest one
 // keeps all its bits however far apart the rows' exponents are.
-// Weights then lie between 2^-119 and 2^100 where they count (b_j is in [-100,
-// 119]), which leaves no room below for the small ones: with v_j = b_j - 23 in
-// place of b_j above, m is 23 lower, the exponential gives 2^(x_j - m) 2^23, and its
-// sum is taken times 2^-23 in the same instruction, so that nothing above 2^-149 is
-// lost. When m moves by more than fp32 spans, l must keep what P and acc may drop
-// (rows of zeros have b_j = -100 and may have all of the weight): l is rescaled by
-// the square root of the factor, twice.
+// The largest weight that counts then is between 2^-119 and 2^100 (b_j is in [-100,
+// 119]), which leaves no room below for smaller ones: the exponential gives 2^23
+// 2^(x_j - m), and its sum is taken times 2^-23 in the instruction that adds, so that
+// nothing above 2^-149 is lost. When m moves by more than fp32 spans, l must keep
+// what P and acc may drop (rows of zeros have b_j = -100 and may have all of the
+// weight): l is rescaled by the square root of the factor, twice. (Both at every
+// step: branching to them where some b_j is large cost 1-4 % more.)
 //
 // Operands are fp16 terms: q' of fp32 rows as two (2^-23 of the row's largest
 // element), of bf16 and fp16 rows as one (exact up to 2^-25 of the largest); P of
@@ -140,14 +140,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The same down to 2^-149.
-__device__ __forceinline__ float ex2_full(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// The weights' shift: 2^23 times a weight is at most 2^(100 + kMargin + 23) < 2^128.
+// 2^kUpBy times a weight is at most 2^(100 + kMargin + 23) < 2^128. (Added after m is
+// taken off: beside a score beyond 2^27 it would be rounded away.)
 constexpr float kUpBy = 23.0f;
 
 // a, b as fp16 in one word (a low).
@@ -463,10 +457,10 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             }
             return r;
         };
-        auto store_exps = [&](const Exps& x, int b) {  // 2^a_j of the 16 positions, then b_j - kUpBy
+        auto store_exps = [&](const Exps& x, int b) {  // 2^a_j of the 16 positions, then b_j
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
-                sE[(b * SUB + u) * 32 + lane] = lane < 16 ? exp2_int(min(max(x.e[u], -126), 127)) : float(x.e[u]) - kUpBy;
+                sE[(b * SUB + u) * 32 + lane] = lane < 16 ? exp2_int(min(max(x.e[u], -126), 127)) : float(x.e[u]);
             }
         };
         Exps ahead{};
@@ -629,7 +623,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
                     const float mn = top > m[nq][i] + kMargin ? top : m[nq][i];
                     const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-                    const float root = ex2_full(0.5f * (m[nq][i] - mu));
+                    const float root = ex2(0.5f * (m[nq][i] - mu));
                     alpha[nq][i] = root * root;
                     m[nq][i] = mn;
                     float sum = 0.f;
@@ -638,7 +632,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const float y = x[u][k] - mu;
-                            sum = fmaf(ex2(y), 0x1p-23f, sum);
+                            sum = fmaf(ex2(y + kUpBy), 0x1p-23f, sum);
                             pw[u][k][i] = ex2(y + vb[u][k]);
                         }
                     l[nq][i] = fmaf(l[nq][i] * root, root, sum);
@@ -766,7 +760,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
             float L = 0.f, f[kWarps];
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) {
-                const float root = ex2_full(0.5f * (ml[k].x - mu));
+                const float root = ex2(0.5f * (ml[k].x - mu));
                 f[k] = root * root;
                 L = fmaf(ml[k].y * root, root, L);
             }

@@ -157,3 +157,28 @@ def test_large_values_whose_scores_grow_slowly(nv, torch, dtype, rows):
     q, k = np.zeros((rows, 1, 64)), np.zeros((ctx, 1, 64))
     q[:, :, 0], k[64:, :, 0] = 1.0, 8 * 7.5 * np.log(2.0)  # 2^7.5 times the weight of the first 64
     Rows(nv, torch, q, k, np.abs(normal(7, ctx, 1, 64)) * 2.0 ** 116, dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,ctx", [(1, 40), (1, 3000)], ids=["short", "long"])
+@pytest.mark.parametrize("power", [14, 28, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_beyond_each_other(nv, torch, dtype, rows, ctx, power, sign):
+    """Scores some 2^power apart: the whole weight is on the largest, exactly."""
+    if dtype == "fp16" and power > 14:
+        power = 15  # the type's range
+    q, k, v = np.zeros((rows, 1, 64)), np.zeros((ctx, 1, 64)), normal(11, ctx, 1, 64)
+    q[:, 0, 0] = sign * 1.3 * 2.0 ** power
+    k[:, 0, 0] = [13 + 2 * (j % 2) + 4 * (j % 5) + (200 if j == ctx // 3 else 0) for j in range(ctx)]
+    k[:, 0, 0] *= 2.0 ** (12 if dtype == "fp16" else 0)
+    x = Rows(nv, torch, q, k, v, dtype, fmt="int8")
+    for r in range(rows):
+        seen = sign * x.k[: ctx - rows + r + 1, 0, 0]
+        best = x.v[: len(seen)][seen == seen.max()].mean(0)
+        off = np.abs(values64(x.out[r]) - best[0])
+        half = {"fp32": 2.0 ** -24, "bf16": 2.0 ** -8, "fp16": 2.0 ** -11}[dtype]
+        n = int((seen == seen.max()).sum())
+        mean = np.abs(x.v[: len(seen)][seen == seen.max()]).mean(0)[0]
+        # equal weights, which the product with V may take rounded: that, the sums' n
+        # additions and the output's rounding
+        assert (off <= half * np.abs(best[0]) + ((2 * n + 16) * 2.0 ** -23 + ref.WEIGHT[dtype]) * mean).all(), r
