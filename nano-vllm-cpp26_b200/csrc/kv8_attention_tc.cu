@@ -85,6 +85,10 @@ constexpr float kMargin = 8.0f;
 // 2^kMargin, a value 2^127.8, and their sums have to stay within fp32. bf16 has the
 // range, and 2^-16 of the smallest value, 2^-109, is a normal number still.
 constexpr float kDownBy = 16.0f;
+// Scores go through one multiply-add, whose exact product can exceed the rounded m by
+// 2^-24 of it: 4 at this size, and infinity as a weight from 2^31 on. Beyond it
+// (warps whose m is, which models' are not) scores are rounded first.
+constexpr float kFarScore = 67108864.0f;  // 2^26
 
 template <int kFormat>
 constexpr int kUp = kFormat == NVLLM_KV8_E4M3 ? 7 : 5;
@@ -487,7 +491,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                     }
                 }
                 // a factor above 0 keeps -inf what it is for rows of zeros
-                const float f = fmaxf(qs * exp2_int(min(max(A - U, -126), 127)), 1.2e-38f);
+                float f = fmaxf(qs * exp2_int(min(max(A - U, -126), 127)), 1.2e-38f);
                 float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
                 for (int k = 4; k < kKeys; k += 8) {
@@ -501,21 +505,29 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
                 const float alpha = ex2_ftz(m - mu);
                 m = mn;
-                if (t > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                    // O must hold the previous tile's products before it is rescaled
-                    if (!wait_all(&ctl->o_full[half][b ^ 1u], ((hn - 1) >> 1) & 1u)) {
-                        ok = false;
-                        break;
-                    }
-                    tc::fence_after_sync();
-#pragma unroll 1
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float ov[32];
-                        tc::tmem_ld32(tO + c * 32u, ov);
-                        tc::tmem_ld_wait();
+                const bool far = fabsf(mu) > kFarScore;
+                if (__any_sync(0xffffffffu, alpha != 1.0f || far)) {  // one vote: it is on every tile's path
+                    if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) ov[k] *= alpha;
-                        tc::tmem_st32(tO + c * 32u, ov);
+                        for (int k = 0; k < kKeys; ++k) sc[k] = __fmul_rn(sc[k], f);
+                        f = 1.0f;
+                    }
+                    if (t > 0) {
+                        // O must hold the previous tile's products before it is rescaled
+                        if (!wait_all(&ctl->o_full[half][b ^ 1u], ((hn - 1) >> 1) & 1u)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; ++c) {
+                            float ov[32];
+                            tc::tmem_ld32(tO + c * 32u, ov);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) ov[k] *= alpha;
+                            tc::tmem_st32(tO + c * 32u, ov);
+                        }
                     }
                 }
                 float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};

@@ -160,7 +160,7 @@ def test_large_values_whose_scores_grow_slowly(nv, torch, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("rows,ctx", [(1, 40), (1, 3000)], ids=["short", "long"])
+@pytest.mark.parametrize("rows,ctx", [(1, 40), (1, 3000), (60, 200)], ids=["short", "long", "chunk"])
 @pytest.mark.parametrize("power", [14, 28, 60])
 @pytest.mark.parametrize("sign", [1, -1])
 def test_scores_far_beyond_each_other(nv, torch, dtype, rows, ctx, power, sign):
