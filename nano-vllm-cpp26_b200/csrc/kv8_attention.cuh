@@ -610,7 +610,9 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const float d = NT == 2 ? s[nq][u][2 * k] + s[nq][u][2 * k + 1] : s[nq][u][2 * k + i];
-                            x[u][k] = (d * ka[u][k]) * qs[nq][i];
+                            // the factors first: a code sum times 2^a alone may leave fp32's
+                            // range (large keys, small queries). Rounded before m is taken off.
+                            x[u][k] = __fmul_rn(d, ka[u][k] * qs[nq][i]);
                             if (ragged) {
                                 const int j = base + u * kSub + g + 8 * k;
                                 const bool see = j <= pos[nq][i] &&

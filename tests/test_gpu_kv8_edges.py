@@ -182,3 +182,11 @@ def test_scores_far_beyond_each_other(nv, torch, dtype, rows, ctx, power, sign):
         # equal weights, which the product with V may take rounded: that, the sums' n
         # additions and the output's rounding
         assert (off <= half * np.abs(best[0]) + ((2 * n + 16) * 2.0 ** -23 + ref.WEIGHT[dtype]) * mean).all(), r
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("power", [-85, 60, 124])
+def test_large_keys_and_small_queries(nv, torch, dtype, rows, power):
+    """Scores of ordinary size from factors far from it."""
+    Rows(nv, torch, normal(8, rows, 2, 128) * 2.0 ** -power, normal(9, 300, 2, 128) * 2.0 ** power, normal(10, 300, 2, 128), dtype).check()
