@@ -410,7 +410,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 x.in = 0;
                 x.blk = seen(j) ? block_at(j, x.in) : -1;
             }
-            x.exps = 0;
+            x.exps = kKv8MinExp;  // of a row of zeros, so that it raises no maximum
             if (x.blk >= 0) {
                 const int8_t* e = lane < 16 ? p.a.k_exps : p.a.v_exps;
                 x.exps = e[int64_t(x.blk) * p.a.exp_block_stride + int64_t(h) * p.a.block_size +

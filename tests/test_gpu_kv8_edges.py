@@ -190,3 +190,19 @@ def test_scores_far_beyond_each_other(nv, torch, dtype, rows, ctx, power, sign):
 def test_large_keys_and_small_queries(nv, torch, dtype, rows, power):
     """Scores of ordinary size from factors far from it."""
     Rows(nv, torch, normal(8, rows, 2, 128) * 2.0 ** -power, normal(9, 300, 2, 128) * 2.0 ** power, normal(10, 300, 2, 128), dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("block", [8, 16])
+@pytest.mark.parametrize("seqs", [[(1, 100), (1, 50)], [(30, 100), (1, 50)]], ids=["decodes", "chunks"])
+def test_bad_block_ids_beside_small_values(nv, torch, dtype, block, seqs):
+    """They count as zero rows whatever the size of the others."""
+    b = Batch(nv, torch, seqs, 2, 1, 64, dtype=dtype, block=block, seed=4)
+    b.arena.v_exp.copy_((b.arena.v_exp.int() - 80).clamp(min=-100))
+    b.v = [v * 2.0 ** -80 for v in b.v]
+    b.tables[0, 2] = -1
+    b.k[0][2 * block : 3 * block] = 0.0
+    b.v[0][2 * block : 3 * block] = 0.0
+    b.call()
+    assert nv.get_last_error() == nv.ERR_BOUNDS
+    b.check()
