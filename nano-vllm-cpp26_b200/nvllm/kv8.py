@@ -243,6 +243,8 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
                                             arena.device)
     elif workspace.get_device() != arena.index:
         raise ValueError(f"workspace must be on the arena's device {arena.device}")
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     st = _call(arena, stream, _lib().nvllm_kv8_attention, out.data_ptr(), _stride(out),
                query.data_ptr(), _stride(query), kind, arena._ref, block_tables.data_ptr(),
                block_tables.shape[1], cu_seqlens_q.data_ptr(), context_lens.data_ptr(), num_seqs,

@@ -125,3 +125,15 @@ def test_calls_run_on_their_tensors_device(world):
     assert world.device == 0
     with pytest.raises(ValueError, match="device"):
         world.kv8.kv8_write(rows, rows, world.arena(0), Tensor(2, dtype=t.int32, device=1), 0)
+
+
+def test_a_workspace_must_be_the_bytes_it_counts(world):
+    """An expanded tensor counts elements that it has no memory for."""
+    t = world.torch
+    good = Tensor(1 << 16, dtype=t.uint8, size=1)
+    world.attention(workspace=good)
+    assert world.calls[-1].args[-3] == 1 << 16
+    n = len(world.calls)
+    with pytest.raises(ValueError, match="workspace.*contiguous"):
+        world.attention(workspace=Tensor(1 << 16, dtype=t.uint8, size=1, contiguous=False))
+    assert len(world.calls) == n
