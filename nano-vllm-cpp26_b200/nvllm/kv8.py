@@ -132,6 +132,12 @@ def _ints(t, name: str, arena: KV8Arena, dim: int = 1):
         raise ValueError(f"{name} must be a contiguous {dim}-d tensor")
 
 
+def _int32(*n: int) -> None:
+    """Refuses arguments that the C ABI's int32 would cut."""
+    if max(n) > 2147483647 or min(n) < -2147483648:
+        raise ValueError("integer arguments must fit 32 bits")
+
+
 def _stride(t) -> int:
     # the stride of a lone row means nothing
     return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
@@ -167,6 +173,7 @@ def _move(what: str, f, key, value, arena: KV8Arena, slot_mapping, layer: int, s
     if _rows(value, "value", width, arena) != kind:
         raise ValueError(f"key and value must have one type, got {key.dtype} and {value.dtype}")
     _ints(slot_mapping, "slot_mapping", arena)
+    _int32(layer, 0)
     n = slot_mapping.numel()
     if key.shape[0] < n or value.shape[0] < n:
         raise ValueError(f"key and value must hold slot_mapping's {n} rows")
@@ -195,6 +202,7 @@ def kv8_read(key, value, arena: KV8Arena, slot_mapping, layer: int, stream=None,
 
 def kv8_workspace_size(num_seqs: int, max_query_len: int, max_context_len: int, num_heads: int,
                        layout: _nv.KVLayout) -> int:
+    _int32(num_seqs, max_query_len, max_context_len, num_heads)
     return int(_lib().nvllm_kv8_attention_workspace_size(num_seqs, max_query_len, max_context_len,
                                                          num_heads, ctypes.byref(layout)))
 
@@ -231,6 +239,7 @@ def kv8_attention(out, query, arena: KV8Arena, block_tables, cu_seqlens_q, conte
     _ints(block_tables, "block_tables", arena, 2)
     _ints(cu_seqlens_q, "cu_seqlens_q", arena)
     _ints(context_lens, "context_lens", arena)
+    _int32(max_query_len, max_context_len, layer, window, sinks)
     num_seqs = context_lens.numel()
     if block_tables.shape[0] != num_seqs or cu_seqlens_q.numel() != num_seqs + 1:
         raise ValueError("block_tables, cu_seqlens_q and context_lens disagree on the sequences")

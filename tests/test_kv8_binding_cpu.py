@@ -137,3 +137,33 @@ def test_a_workspace_must_be_the_bytes_it_counts(world):
     with pytest.raises(ValueError, match="workspace.*contiguous"):
         world.attention(workspace=Tensor(1 << 16, dtype=t.uint8, size=1, contiguous=False))
     assert len(world.calls) == n
+
+
+BIG = 1 << 32
+
+
+@pytest.mark.parametrize("arg", ["max_query_len", "max_context_len", "layer", "window", "sinks"])
+@pytest.mark.parametrize("value", [BIG, BIG + 5, 1 << 31, -BIG + 5])
+def test_attention_refuses_what_32_bits_do_not_hold(world, arg, value):
+    """The C ABI takes int32, and ctypes drops the rest without a word."""
+    with pytest.raises(ValueError, match="32 bits"):
+        world.attention(**{arg: value})
+    assert not world.calls
+    world.attention(window=(1 << 31) - 1, sinks=(1 << 31) - 1)
+    world.attention(layer=-1)  # the library's to refuse
+    assert len(world.calls) == 2
+
+
+@pytest.mark.parametrize("value", [BIG, -BIG + 1])
+def test_moves_and_sizes_refuse_what_32_bits_do_not_hold(world, value):
+    t = world.torch
+    rows, slots = Tensor(2, 128, dtype=t.float32), Tensor(2, dtype=t.int32)
+    for f in (world.kv8.kv8_write, world.kv8.kv8_read):
+        with pytest.raises(ValueError, match="32 bits"):
+            f(rows, rows, world.arena(), slots, value)
+    for i in range(4):
+        args = [1, 1, 1, 2]
+        args[i] = value
+        with pytest.raises(ValueError, match="32 bits"):
+            world.kv8.kv8_workspace_size(*args, world.layout)
+    assert not world.calls
