@@ -140,7 +140,7 @@ def _int32(*n: int) -> None:
 
 def _stride(t) -> int:
     # the stride of a lone row means nothing
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
 
 
 def _call(arena: KV8Arena, stream, f, *args) -> int:

@@ -167,3 +167,14 @@ def test_moves_and_sizes_refuse_what_32_bits_do_not_hold(world, value):
         with pytest.raises(ValueError, match="32 bits"):
             world.kv8.kv8_workspace_size(*args, world.layout)
     assert not world.calls
+
+
+def test_a_lone_row_has_no_stride(world):
+    """One row sliced out of a buffer whose rows are not a multiple of 16 bytes apart."""
+    t = world.torch
+    q, out = (Tensor(1, 128, dtype=t.bfloat16, size=2, stride=(s, 1)) for s in (387, 1))
+    world.attention(query=q, out=out)
+    assert (world.calls[-1].args[1], world.calls[-1].args[3]) == (128, 128)
+    q, out = (Tensor(2, 128, dtype=t.bfloat16, size=2, stride=(s, 1)) for s in (384, 136))
+    world.attention(query=q, out=out)
+    assert (world.calls[-1].args[1], world.calls[-1].args[3]) == (136, 384)
