@@ -272,12 +272,13 @@ int nvllm_device_status_word(const uint32_t** word);
  * rows). 0 if none was seen. */
 uint32_t nvllm_last_status_word(void);
 
-/* With that word, where the first bounded wait that gave up was: info[0] its
+/* With that word, where the first bounded wait that gave up was, for the kernels
+ * of bits 12, 14, 15 and 16 (the others set their bit alone): info[0] its
  * kernel bits (as above, | 1), info[1] a kernel-specific code (the role,
  * barrier and pipeline stage of the wait), info[2] the CTA, info[3] the low
  * word of the mbarrier at the time. For the two cross-GPU flag waits (bits 14
  * and 15) info[1] is the flag value awaited and info[3] the value last read.
- * All 0 when no wait gave up. */
+ * All 0 when none of theirs gave up. */
 int nvllm_last_timeout_info(uint32_t* info);
 
 /* Static string for a status code. */

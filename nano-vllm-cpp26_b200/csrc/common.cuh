@@ -24,9 +24,20 @@ enum : uint32_t {
     kStatusInKv8Tc = 1u << 16,
 };
 
+// Fills a timeout record (g_timeout_info's words) unless an earlier wait did.
+__device__ __forceinline__ void record_timeout_at(uint32_t* info, uint32_t site, uint32_t where,
+                                                  const uint64_t* bar) {
+    if (atomicCAS(&info[0], 0u, site | 1u) == 0u) {
+        info[1] = where;
+        info[2] = blockIdx.x;
+        info[3] = static_cast<uint32_t>(*reinterpret_cast<const volatile uint64_t*>(bar));
+        __threadfence();
+    }
+}
+
 // A file compiled on its own (NVLLM_WHOLE_PROGRAM, for the register splits that
-// relocatable code does not allow) cannot name them: its kernels take the status
-// word's address.
+// relocatable code does not allow) cannot name these two: its kernels take their
+// addresses.
 #ifndef NVLLM_WHOLE_PROGRAM
 extern __device__ uint32_t g_status;
 // Where the first bounded wait that gave up was: {site bits, where code (set by
@@ -37,12 +48,7 @@ extern __device__ uint32_t g_timeout_info[4];
 __device__ __forceinline__ void raise_status(uint32_t bits) { atomicOr(&g_status, bits); }
 
 __device__ __forceinline__ void record_timeout(uint32_t site, uint32_t where, const uint64_t* bar) {
-    if (atomicCAS(&g_timeout_info[0], 0u, site | 1u) == 0u) {
-        g_timeout_info[1] = where;
-        g_timeout_info[2] = blockIdx.x;
-        g_timeout_info[3] = static_cast<uint32_t>(*reinterpret_cast<const volatile uint64_t*>(bar));
-        __threadfence();
-    }
+    record_timeout_at(g_timeout_info, site, where, bar);
 }
 
 // The same record for a cross-GPU flag wait that gave up: the value awaited
@@ -134,6 +140,30 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
     }
 }
 #endif  // NVLLM_WHOLE_PROGRAM
+
+// Bounded wait that also gives up once another role has. The first of a CTA to time
+// out leaves its barrier's address in *abort; report_abort writes that out when the
+// roles have met (a report at every wait cost the prompt kernel of the 8-bit cache
+// 1.5 %, a code that names the warp and the phase too 8 %: registers).
+__device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parity, uint32_t* abort) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile uint32_t*>(abort)) return false;
+        if (global_ns() - t0 > kWaitLimitNs) {
+            atomicCAS(abort, 0u, smem_addr(bar));
+            return false;
+        }
+    }
+}
+// bars: what the record's code (the barrier's place) counts from.
+__device__ __forceinline__ void report_abort(uint32_t* status, uint32_t* info, uint32_t site, uint32_t abort,
+                                             const uint64_t* bars) {
+    const uint32_t place = (abort - smem_addr(bars)) / 8;
+    atomicOr(status, kStatusTimeout | site);
+    record_timeout_at(info, site, place, bars + place);
+}
 
 // ---- bulk async copy global -> shared (TMA, no multicast) -----------------
 // dst and src 16-byte aligned, bytes a multiple of 16.

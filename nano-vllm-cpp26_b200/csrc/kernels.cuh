@@ -14,6 +14,9 @@ namespace nvllm {
 int validate_layout(const nvllm_kv_layout* lay);
 ArenaGeom make_geom(const nvllm_kv_layout* lay);
 
+// Device addresses of the status word and the timeout record on the current device.
+cudaError_t device_report(uint32_t** status, uint32_t** timeout_info);
+
 // Work items produced by the plan kernel.
 //   decode item  (seq, split):  positions [split*P, min((split+1)*P, ctx))
 //   prefill item (seq, tile):   query rows [tile*QT, min((tile+1)*QT, q_len))

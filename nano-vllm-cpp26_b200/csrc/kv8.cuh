@@ -61,7 +61,8 @@ struct Kv8AttnParams {
     int32_t window;
     int32_t sinks;
     float qk_scale_log2;  // softmax scale * log2(e)
-    uint32_t* status;     // the device status word (whole-program kernels)
+    uint32_t* status;        // the device status word (whole-program kernels)
+    uint32_t* timeout_info;  // and the timeout record
     bool fp16;            // 16-bit rows are fp16, not bf16 (kernels that serve both)
 };
 

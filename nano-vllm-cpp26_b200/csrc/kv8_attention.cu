@@ -98,9 +98,8 @@ cudaError_t launch_kv8_attention(const Kv8AttnParams& all, int32_t dtype, int32_
         cudaError_t e = w.groups > 0 ? cudaSuccess : launch_kv8_plan(p, w, stream);
         if (e != cudaSuccess) return e;
         if (w.groups == 0 && kv8_tc_supported(dtype, g.head_dim)) {
-            const uint32_t* word = nullptr;
-            if (nvllm_device_status_word(&word) != NVLLM_OK) return cudaErrorInvalidSymbol;
-            p.status = const_cast<uint32_t*>(word);
+            e = device_report(&p.status, &p.timeout_info);
+            if (e != cudaSuccess) return e;
             e = launch_kv8_tc(p, w, dtype, format, stream);
         } else if (dtype == NVLLM_DTYPE_FP32) {
             e = launch_rows(p, w, true, format, stream);

@@ -47,8 +47,8 @@
 // of the last round cut 1.30. A step of 128 keys with one S per half was slower, 1.69
 // against 1.44: S is then exposed behind the softmax.
 //
-// Every wait is bounded; on a timeout the CTA records NVLLM_ERR_TIMEOUT, lets its
-// MMAs finish and frees its TMEM.
+// Every wait is bounded; on a timeout the CTA lets its MMAs finish, reports
+// NVLLM_ERR_TIMEOUT with the wait's record and frees its TMEM.
 #include <algorithm>
 #include <type_traits>
 
@@ -123,7 +123,7 @@ struct Control {
     int32_t large[kRaw];        // some V exponent of a key tile is above 7
     uint32_t tmem_base;
     int32_t items[2];
-    int32_t abort;
+    uint32_t abort;             // address of the barrier whose wait gave up first, or 0
 };
 
 template <int HD>
@@ -148,19 +148,8 @@ struct Shape {
     static constexpr int LOAD_STEP = 32 / PIECES;              // rows that a loader copies at once
 };
 
-// Bounded wait that also gives up once another role has aborted.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl, uint32_t* status) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*reinterpret_cast<volatile int32_t*>(&ctl->abort)) return false;
-        if (global_ns() - t0 > kWaitLimitNs) {
-            atomicOr(status, kStatusTimeout | kStatusInKv8Tc);
-            atomicExch(&ctl->abort, 1);
-            return false;
-        }
-    }
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Control* ctl) {
+    return mbar_wait_or_abort(bar, parity, &ctl->abort);
 }
 
 __device__ __forceinline__ float ex2_ftz(float x) {
@@ -339,7 +328,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     bool issued_mma = false;   // MMA warp
 
     auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl, p.status));
+        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ctl));
     };
     // One arrival for the warp, after all its lanes' writes (each fenced by its lane).
     auto warp_arrive = [&](uint64_t* bar) {
@@ -352,7 +341,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     // item's end.
     auto publish = [&](uint32_t j, int it) -> bool {
         const uint32_t slot = j & 1u;
-        if (j >= 2 && !wait_or_abort(&ctl->item_free[slot], ((j >> 1) - 1) & 1u, ctl, p.status)) return false;
+        if (j >= 2 && !wait_or_abort(&ctl->item_free[slot], ((j >> 1) - 1) & 1u, ctl)) return false;
         ctl->items[slot] = it;
         mbar_arrive(&ctl->item_full[slot]);
         return true;
@@ -370,7 +359,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
         int it = -1;
         if (warp == kLoadWarp) {
             if (lane == 0) {
-                if (!*reinterpret_cast<volatile int32_t*>(&ctl->abort)) {
+                if (!*reinterpret_cast<volatile uint32_t*>(&ctl->abort)) {
                     it = atomicAdd(&w.counters->next, 1);
                     if (it >= total) it = -1;
                 }
@@ -380,7 +369,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
         } else {
             it = take(j);
         }
-        return *reinterpret_cast<volatile int32_t*>(&ctl->abort) ? -1 : it;
+        return *reinterpret_cast<volatile uint32_t*>(&ctl->abort) ? -1 : it;
     };
     struct Job {
         Kv8Item item;
@@ -859,7 +848,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
             const uint32_t tS = uniform(tmem) + 128u * i;
             const uint32_t tO = uniform(tmem) + 256u + 128u * i;
             auto both = [&](uint64_t* x, uint32_t px, uint64_t* y, uint32_t py) -> bool {
-                return __all_sync(0xffffffffu, wait_or_abort(x, px, ctl, p.status) && wait_or_abort(y, py, ctl, p.status));
+                return __all_sync(0xffffffffu, wait_or_abort(x, px, ctl) && wait_or_abort(y, py, ctl));
             };
             uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;  // stage and phase of the next S and O
             uint32_t s_n = 0, o_n = 0;                        // S and O of this half so far
@@ -948,6 +937,10 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
     }
     tc::fence_before_sync();
     __syncthreads();
+    if (tid == 0 && ctl->abort != 0) {
+        // the record's code: the barrier's place in the control block
+        report_abort(p.status, p.timeout_info, kStatusInKv8Tc, ctl->abort, reinterpret_cast<uint64_t*>(ctl));
+    }
     if (warp == kMmaWarp) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, kTmemCols);

@@ -52,6 +52,12 @@ ArenaGeom make_geom(const nvllm_kv_layout* lay) {
     return g;
 }
 
+cudaError_t device_report(uint32_t** status, uint32_t** timeout_info) {
+    cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(status), g_status);
+    if (e == cudaSuccess) e = cudaGetSymbolAddress(reinterpret_cast<void**>(timeout_info), g_timeout_info);
+    return e;
+}
+
 WorkspaceLayout workspace_layout(int32_t num_seqs, int32_t max_query_len, int32_t max_context_len,
                                  int32_t num_heads, int32_t head_dim) {
     WorkspaceLayout w{};
