@@ -175,8 +175,13 @@ int nvllm_paged_attention_head_split(const nvllm_head_split* hs, const float* qu
  */
 enum nvllm_dtype { NVLLM_DTYPE_FP32 = 0, NVLLM_DTYPE_BF16 = 1, NVLLM_DTYPE_FP16 = 2 };
 enum nvllm_kv8_format {
-    NVLLM_KV8_E4M3 = 0, /* 8-bit float: relative error <= 2^-4 of each value */
-    NVLLM_KV8_INT8 = 1  /* 8-bit integer: absolute error <= max|x| / 127 of the row */
+    /* 8-bit float: relative error <= 2^-4 of values from 2^-6 2^e on, absolute error
+     * <= 2^-10 2^e of smaller ones (max|x| of the row is above 224 * 2^e) */
+    NVLLM_KV8_E4M3 = 0,
+    /* 8-bit integer: absolute error <= max|x| / 127 of the row */
+    NVLLM_KV8_INT8 = 1
+    /* (a row whose max|x| is below M * 2^-100 has e = -100: absolute error <= half a
+     * code of that) */
 };
 
 /* Arenas on the device, owned by the caller. Codes: [num_blocks, num_layers,
@@ -232,14 +237,22 @@ size_t nvllm_kv8_attention_workspace_size(int32_t num_seqs, int32_t max_query_le
  * j > p - window or j < sinks (a sliding window of `window` positions, itself
  * included, and the sequence's first `sinks` positions); window 0: all j <= p
  * (sinks is then not used). Blocks of which no row sees a position may have been
- * freed: their table entries are not read. Positions whose block id lies outside the arena
- * count as zero rows and raise NVLLM_ERR_BOUNDS; a sequence whose metadata
- * contradicts the maxima is skipped (its rows stay as they were) and raises
- * NVLLM_ERR_INVALID in nvllm_get_last_error. Rows that belong to no sequence
- * are not touched. At most 65535 sequences. The workspace (256-byte aligned; one
- * sized for larger maxima of the same layout and query heads serves) is
- * overwritten by each call: calls that may overlap on the GPU need one each. A
- * first call on a device belongs outside stream capture: it loads the kernels. */
+ * freed: their table entries are not read. Positions whose block id lies outside
+ * the arena count as zero rows and raise NVLLM_ERR_BOUNDS; a sequence whose
+ * metadata contradicts the maxima is skipped (its rows stay as they were) and
+ * raises NVLLM_ERR_INVALID in nvllm_get_last_error. Rows that belong to no
+ * sequence are not touched. At most 65535 sequences.
+ *
+ * Sums are taken in 32 bits: scores (scale * q . K) have to stay below 2^25 in size,
+ * and a context's length times its largest |V| below 2^127. A softmax weight is
+ * rounded before its product with V: for fp32 rows to 22 bits, for bf16 rows to 8 in
+ * prompts and chunks at head_dim 64 and 128 and to 11 elsewhere, for fp16 rows to 16
+ * and 11.
+ *
+ * The workspace (256-byte aligned; one sized for larger maxima of the same layout
+ * and query heads serves) is overwritten by each call: calls that may overlap on
+ * the GPU need one each. A first call on a device belongs outside stream capture:
+ * it loads the kernels. */
 int nvllm_kv8_attention(void* out, int64_t out_stride, const void* query, int64_t query_stride,
                         int32_t dtype, const nvllm_kv8_arena* arena,
                         const int32_t* block_tables, int32_t max_blocks_per_seq,

@@ -1,5 +1,6 @@
 """The Python binding of the 8-bit cache without a GPU: which stream and device a
-call and its default workspace are on, with stand-ins for tensors and torch.cuda."""
+call and its default workspace are on, with stand-ins for tensors and torch.cuda;
+and the errors that the header states of the formats."""
 import contextlib
 from types import SimpleNamespace
 
@@ -178,3 +179,21 @@ def test_a_lone_row_has_no_stride(world):
     q, out = (Tensor(2, 128, dtype=t.bfloat16, size=2, stride=(s, 1)) for s in (384, 136))
     world.attention(query=q, out=out)
     assert (world.calls[-1].args[1], world.calls[-1].args[3]) == (136, 384)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_the_stated_errors_of_the_formats(fmt):
+    """What include/nvllm.h says of each format's error, over rows whose elements are
+    far apart; for E4M3 a relative error alone is not true of the small ones."""
+    import numpy as np
+    import kv8_ref as ref
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((400, 64)) * 2.0 ** rng.integers(-20, 1, (400, 64)) * 2.0 ** rng.integers(-40, 40, (400, 1))
+    codes, e = ref.quantise(x, fmt)
+    off, step = np.abs(ref.dequantise(codes, e, fmt) - x), 2.0 ** e[:, None].astype(np.float64)
+    if fmt == "e4m3":
+        assert (off <= np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * step)).all()
+        assert (off[np.abs(x) >= 2.0 ** -6 * step] <= 2.0 ** -4 * np.abs(x)[np.abs(x) >= 2.0 ** -6 * step]).all()
+        assert (off > 2.0 ** -4 * np.abs(x)).any()
+    else:
+        assert (off <= np.abs(x).max(1, keepdims=True) / 127).all()
