@@ -87,7 +87,7 @@ constexpr float kMargin = 8.0f;
 constexpr float kDownBy = 16.0f;
 // Scores go through one multiply-add, whose exact product can exceed the rounded m by
 // 2^-24 of it: 4 at this size, and infinity as a weight from 2^31 on. Beyond it
-// (warps whose m is, which models' are not) scores are rounded first.
+// (rows whose m is, which models' are not) scores are rounded first.
 constexpr float kFarScore = 67108864.0f;  // 2^26
 
 template <int kFormat>
@@ -497,9 +497,11 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 const bool far = fabsf(mu) > kFarScore;
                 if (__any_sync(0xffffffffu, alpha != 1.0f || far)) {  // one vote: it is on every tile's path
                     if (__any_sync(0xffffffffu, far)) {
+                        // (of these rows alone: the others keep their bits)
+                        const float g = far ? f : 1.0f;
 #pragma unroll
-                        for (int k = 0; k < kKeys; ++k) sc[k] = __fmul_rn(sc[k], f);
-                        f = 1.0f;
+                        for (int k = 0; k < kKeys; ++k) sc[k] = __fmul_rn(sc[k], g);
+                        f = far ? 1.0f : f;
                     }
                     if (t > 0) {
                         // O must hold the previous tile's products before it is rescaled

@@ -206,3 +206,29 @@ def test_bad_block_ids_beside_small_values(nv, torch, dtype, block, seqs):
     b.call()
     assert nv.get_last_error() == nv.ERR_BOUNDS
     b.check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("seqs", [[(1, 1), (1, 70), (1, 700), (1, 3000)], [(40, 200), (1, 40), (90, 90)]], ids=["decodes", "chunks"])
+@pytest.mark.parametrize("window", [0, 50])
+def test_queries_that_are_not_numbers(nv, torch, dtype, seqs, window):
+    """A NaN or an infinity makes its own row and head NaN and leaves the others."""
+    b = Batch(nv, torch, seqs, 4, 2, 64, dtype=dtype, seed=14, window=window, sinks=3)
+    q = b.query.reshape(-1, 4, 64)
+    clean = b.query.clone()
+    rows = q.shape[0]
+    bad = [(0, 1, np.nan), (rows // 2, 3, np.inf), (rows - 1, 0, -np.inf)]
+    for r, h, x in bad:
+        q[r, h, 5] = x
+    b.call()
+    out = b.out.reshape(-1, 4, 64)
+    for r, h, _ in bad:
+        assert out[r, h].isnan().all()
+    b.query.copy_(clean)
+    good = b.out.clone()
+    b.out.fill_(9.0)
+    b.call()
+    b.check()
+    for r, h, _ in bad:
+        good.reshape(-1, 4, 64)[r, h] = out[r, h]
+    assert torch.equal(good, b.out)
