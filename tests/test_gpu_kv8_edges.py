@@ -2,6 +2,8 @@
 tiles alternate in size, workspaces and streams left to the call, exponents at
 the ends of their range, queries that are not numbers. The batch, the 64-bit
 answer and the derived tolerance are those of test_gpu_kv8 and kv8_ref."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -232,3 +234,70 @@ def test_queries_that_are_not_numbers(nv, torch, dtype, seqs, window):
     for r, h, _ in bad:
         good.reshape(-1, 4, 64)[r, h] = out[r, h]
     assert torch.equal(good, b.out)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("by", [12, 40, 90])
+def test_prompts_with_some_large_value_exponents(nv, torch, hd, by):
+    """E4M3 exponents above 7 at some positions of a key tile, at all, and at none."""
+    b = Batch(nv, torch, [(40, 200), (130, 130)], 8, 2, hd, dtype="bf16", seed=hd)
+    for s, (_, ctx) in enumerate(b.seqs):
+        for j in [*range(3, 64, 7), *range(64, 128)]:
+            blk = int(b.tables[s, j // 16])
+            b.arena.v_exp[blk, b.layer, :, j % 16] += by + (3 if j % 2 else 0)
+            b.v[s][j] *= 2.0 ** (by + (3 if j % 2 else 0))
+    assert int(b.arena.v_exp[int(b.tables[0, 4]), b.layer].min()) > 0
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_fp16_prompts_keep_two_terms_of_a_weight(nv, torch, hd, fmt, monkeypatch):
+    """Two bf16 terms leave at most 2^-8 of 2^-8 of a weight, not one fp16's 2^-11."""
+    monkeypatch.setitem(ref.WEIGHT, "fp16", 2.0 ** -16)
+    b = Batch(nv, torch, [(70, 300), (40, 40), (9, 900)], 8, 2, hd, fmt=fmt, dtype="fp16", seed=3)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("dtype,hd", [("fp16", 64), ("fp16", 128), ("fp32", 32), ("bf16", 32), ("fp32", 256), ("fp16", 256)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 4), (100, 70)])
+@pytest.mark.parametrize("seqs", [[(1, 1), (1, 130), (1, 513)], [(5, 5), (33, 70), (130, 300)]], ids=["decodes", "chunks"])
+def test_windows_of_other_types_and_head_dims(nv, torch, dtype, hd, window, sinks, seqs):
+    b = Batch(nv, torch, seqs, 4, 2, hd, dtype=dtype, window=window, sinks=sinks, seed=window)
+    b.call()
+    b.check()
+
+
+def test_two_host_threads(nv, torch):
+    """Calls from two threads, each with its stream and workspace."""
+    bs = [Batch(nv, torch, s, 4, 2, 64, dtype=d, seed=21 + i)
+          for i, (s, d) in enumerate([([(1, 900), (1, 40)], "bf16"), ([(60, 300), (1, 700)], "fp16")])]
+    for b in bs:
+        b.call()
+    torch.cuda.synchronize()
+    want = [b.out.clone() for b in bs]
+    errors = []
+
+    def work(b, w):
+        try:
+            st = torch.cuda.Stream()
+            ws = nv.kv8_alloc_workspace(len(b.seqs), b.max_new, b.max_ctx, 4, b.arena.layout)
+            torch.cuda.synchronize()
+            for _ in range(50):
+                out = torch.full_like(w, 9.0)
+                st.wait_stream(torch.cuda.current_stream())
+                b.call(out=out, stream=st, workspace=ws)
+                st.synchronize()
+                assert torch.equal(out, w)
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=x) for x in zip(bs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for b in bs:
+        b.check()
