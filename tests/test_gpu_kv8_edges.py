@@ -301,3 +301,13 @@ def test_two_host_threads(nv, torch):
     assert not errors, errors
     for b in bs:
         b.check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(1500, 0), (2000, 700), (3000, 5)])
+@pytest.mark.parametrize("seqs", [[(1, 6000), (1, 1400), (1, 2300)], [(90, 5000), (1, 4000), (300, 300)]], ids=["decodes", "chunks"])
+def test_windows_that_are_cut(nv, torch, dtype, window, sinks, seqs):
+    """Windows of many chunks, shared out over CTAs and merged, the sinks' part among them."""
+    b = Batch(nv, torch, seqs, 4, 1, 64, dtype=dtype, window=window, sinks=sinks, seed=sinks)
+    b.call()
+    b.check()
