@@ -93,7 +93,6 @@ struct Kv8Counters {
     int32_t next;    // cursor over items x KV heads
     int32_t items;
     int32_t merges;
-    int32_t slots;
 };
 struct Kv8Work {
     Kv8Counters* counters;

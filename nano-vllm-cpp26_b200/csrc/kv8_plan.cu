@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) *w.counters = Kv8Counters{0, n_items, n_merges, n_slots};
+    if (threadIdx.x == 0) *w.counters = Kv8Counters{0, n_items, n_merges};
 }
 
 // out = sum_k acc_k 2^(m_k - M) / sum_k l_k 2^(m_k - M), M = max_k m_k: a warp per
