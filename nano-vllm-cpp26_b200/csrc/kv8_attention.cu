@@ -41,15 +41,25 @@ Kv8Work self_work(int nq, int32_t dtype, bool snap, const ArenaGeom& g) {
     return w;
 }
 
-// seen: most positions that a tile sees. Cutting a sequence costs its partials and
-// the merge (7 us of a call of 40): up to 512 positions it never pays, up to 1280
-// only where the sequences do not fill the GPU.
+// Sequences that see at most this many positions are not cut: a cut costs its partials
+// and the merge. Both sides measured, whole | cut, us, bf16 head_dim 128 (2048 units:
+// fp32):
+//   seen                          512         1024        1280        2048        4096
+//   8 (sequence, KV head) units   16.4 | 40   22.5 | 40   26.6 | 41   36.9 | 38   61 | 46
+//   32                            18.4 | 26   24.6 | 32   28.7 | 26   38.9 | 38   70 | 43
+//   128                           20.5 | 24   30.7 | 34   34.8 | 34   49.2 | 40   84 | 54
+//   256                           26.6 | 34   36.9 | 42   43.0 | 44   55.4 | 56   92 | 82
+//   2048                          76 | 81     121 | 124   145 | 147   210 | 214   385 | 388
+constexpr int kWholeFew = 1280;   // where the units are fewer than the SMs
+constexpr int kWholeMany = 2048;
+
+// seen: most positions that a tile sees.
 Kv8Work work_for(int32_t max_query_len, int64_t seen, int64_t units, int32_t group, int32_t dtype,
                  const ArenaGeom& g) {
     const int one = rows_of_tile(dtype);
     const int64_t rows = int64_t(max_query_len) * group;
     const int nq = columns_for(rows, one, g.head_dim);
-    if (rows <= nq * one) return self_work(nq, dtype, seen <= (units >= kKv8Sms ? 1280 : 512), g);
+    if (rows <= nq * one) return self_work(nq, dtype, seen <= (units >= kKv8Sms ? kWholeMany : kWholeFew), g);
     if (kv8_tc_supported(dtype, g.head_dim)) return kv8_tc_work();
     Kv8Work w{};
     w.tile_rows = nq * one;
@@ -70,7 +80,7 @@ size_t kv8_attention_workspace(int32_t num_seqs, int32_t max_query_len, int32_t 
         Kv8Work w = work_for(max_query_len, max_context_len, 0, group, dtype, g);
         n = std::max(n, kv8_work_layout(w, nullptr, num_seqs, max_query_len, max_context_len, group, g));
         for (int q = 1; q <= columns_for(int64_t(max_query_len) * group, rows_of_tile(dtype), g.head_dim); q *= 2) {
-            Kv8Work self = self_work(q, dtype, max_context_len <= 512, g);
+            Kv8Work self = self_work(q, dtype, max_context_len <= kWholeFew, g);
             n = std::max(n, kv8_work_layout(self, nullptr, num_seqs, 1, max_context_len, 1, g));
         }
     }
