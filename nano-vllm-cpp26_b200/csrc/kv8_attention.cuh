@@ -21,7 +21,8 @@
 // Operands are fp16 terms: q' of fp32 rows as two (2^-23 of the row's largest
 // element), of bf16 and fp16 rows as one (exact up to 2^-25 of the largest); P of
 // fp32 rows as two terms (2^-22), of others as one (2^-11, no more than the
-// output's own rounding).
+// output's own rounding: bf16 outputs are 1.7e-3 of their norm from 64 bits, as with
+// P in fp32).
 //
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
 // positions and dims fill the MMA's 16 rows and the few query rows its 8 columns:
@@ -43,8 +44,11 @@
 // joined through shared memory at the end of a run.
 //
 // Measured on B200: 64 sequences of 512-4096 positions, 32 heads x 128, fp32 rows:
-// 230-245 us, up to 5.3 TB/s (0.81 of the copy rate), latency-bound at 47 % issue with
-// 12 warps an SM; 4 x 32768 positions, 32 heads over 8, bf16 rows: 82 us.
+// 244-247 us, 5.0 TB/s (0.76 of the copy rate), latency-bound at 45 % issue with 12
+// warps an SM; 4 x 32768 positions, 32 heads over 8, bf16 rows: 82 us, 66 of them here
+// and the rest the merge. Few (sequence, KV head) units at a long context are the
+// merge's (kv8_plan.cu): one sequence of 32768, 32 heads over 8, 71 us for 10 us of
+// bytes; of 131072, 8 heads on one, 372 us.
 // The order with query rows on the MMA's 16 rows took 518 us for the first, the
 // transposed one with fragments loaded straight into registers 280.
 #pragma once

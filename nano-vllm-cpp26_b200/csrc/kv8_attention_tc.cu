@@ -16,7 +16,8 @@
 // is exact for rows within 2^22 of the tile's largest (2^29 for INT8) and beyond
 // that off by 2^-36 of the largest: a factor below fp16's range is taken in two
 // steps, of which only the last rounds. P is rounded to bf16, half a step of which is
-// the output's own; for fp16 rows, whose step is finer, P is two bf16 terms.
+// the output's own (outputs are 2.4e-3 of their norm from 64 bits, 1.7e-3 with P in
+// fp32); for fp16 rows, whose step is finer, P is two bf16 terms.
 //
 // One CTA per SM, 20 warps in 5 warpgroups:
 //   warps 0-3, 4-7  softmax of the tile's first and second 128 rows: a thread owns
@@ -40,8 +41,8 @@
 // 2400: MMAs on different accumulators have no order of their own, so the S that
 // takes P's place waits until O is complete, and an S of N = 64 is paced by Q's
 // re-reads from shared memory (66 cycles in place of 32).
-// Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.19
-// ms, 812 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 128 us. On the way:
+// Measured on B200: 4096 rows at position 16384, 32 heads over 8 x 128, bf16: 1.21
+// ms, 797 TFLOP/s; 8191 rows, window 1000, 16 heads over 4 x 64: 128 us. On the way:
 // one MMA warp for both halves 1.57 ms (its own instructions paced it), four
 // converter warps that also loaded 1.55, factors written a tile late 1.44, no tile
 // of the last round cut 1.30. A step of 128 keys with one S per half was slower, 1.69

@@ -15,7 +15,8 @@
 // values of K and the same 16 of V (one 16-byte store of codes each), hd / 16
 // neighbouring lanes share a row and find its maximum by shuffles; all of a
 // thread's loads are in flight before the first is used. Measured on B200, 10229
-// tokens of 32 x 128 fp32: 70 us, 6.0 TB/s (0.92 of the copy rate).
+// tokens of 32 x 128 fp32: 71 us, 5.9 TB/s (0.90 of the copy rate); 65536 of 8 x 128
+// bf16: 90-98 us, 4.1-4.5 TB/s.
 #include "kv8.cuh"
 
 namespace nvllm {
@@ -165,8 +166,9 @@ kv8_write_kernel(const Kv8Arena a, const Kv8Rows r) {
 
 // The read's pieces are 16 bytes of output (4 or 8 values), so that a warp's stores
 // are whole lines; a thread takes kReads of them, kThreads apart, of K and of V.
-// Measured on B200, 32768 rows of 32 x 128 to fp32: 262 us, 5.1 TB/s (four pieces a
-// thread 274; the write's pieces, four strided 16-byte stores of fp32, 288).
+// Measured on B200, 32768 rows of 32 x 128 to fp32: 261 us, 5.1 TB/s (four pieces a
+// thread 274; the write's pieces, four strided 16-byte stores of fp32, 288); 65536 of
+// 8 x 128 to bf16: 84 us, 4.8 TB/s.
 constexpr int kReads = 2;
 
 template <typename T, int kFormat, bool kVec>

@@ -168,7 +168,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8AttnPar
 }
 
 // out = sum_k acc_k 2^(m_k - M) / sum_k l_k 2^(m_k - M), M = max_k m_k: a warp per
-// (cut tile, KV head, row), parts in order.
+// (cut tile, KV head, row), parts in order. Without a plan the list has an entry for
+// every range, most of them empty, and the grid is that of the tiles: with few
+// (sequence, KV head) units each warp steps through many entries, which is most of
+// the call (1 x 16384 positions, one head, fp32: 126 us).
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p, const Kv8Work w) {
     constexpr int PER = HD / 32;
