@@ -11,9 +11,9 @@
 // the size of contributions (not of weights) P is in [0, 1] and the largest one
 // keeps all its bits however far apart the rows' exponents are.
 // The largest weight that counts then is between 2^-119 and 2^100 (b_j is in [-100,
-// 119]), which leaves no room below for smaller ones: the exponential gives 2^23
-// 2^(x_j - m), and its sum is taken times 2^-23 in the instruction that adds, so that
-// nothing above 2^-149 is lost. When m moves by more than fp32 spans, l must keep
+// 119]), which leaves no room below for smaller ones: the exponential gives 2^20
+// 2^(x_j - m), and its sum is taken times 2^-20 in the instruction that adds, so that
+// nothing above 2^-146 is lost. When m moves by more than fp32 spans, l must keep
 // what P and acc may drop (rows of zeros have b_j = -100 and may have all of the
 // weight): l is rescaled by the square root of the factor, twice. (Both at every
 // step: branching to them where some b_j is large cost 1-4 % more.)
@@ -144,9 +144,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// 2^kUpBy times a weight is at most 2^(100 + kMargin + 23) < 2^128. (Added after m is
-// taken off: beside a score beyond 2^27 it would be rounded away.)
-constexpr float kUpBy = 23.0f;
+// 2^kUpBy times a weight is at most 2^(100 + kMargin + 2 + 20) < 2^128 (2: half a step
+// of the largest scores, by which m is off). Added after m is taken off: beside a score
+// beyond 2^27 it would be rounded away.
+constexpr float kUpBy = 20.0f;
 
 // a, b as fp16 in one word (a low).
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
@@ -638,7 +639,7 @@ kv8_attention_kernel(const Kv8AttnParams p, const Kv8Work w) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const float y = x[u][k] - mu;
-                            sum = fmaf(ex2(y + kUpBy), 0x1p-23f, sum);
+                            sum = fmaf(ex2(y + kUpBy), 0x1p-20f, sum);
                             pw[u][k][i] = ex2(y + vb[u][k]);
                         }
                     l[nq][i] = fmaf(l[nq][i] * root, root, sum);

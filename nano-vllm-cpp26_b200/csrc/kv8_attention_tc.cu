@@ -866,7 +866,7 @@ kv8_attention_tc_kernel(const Kv8AttnParams p, const Kv8Work w) {
                 // others this warp and the half's softmax each run ahead of the other by up
                 // to two items, and a phase per item would be mistaken for another's. The
                 // softmax cannot leave an item of its half without this warp's S, so neither
-                // is ever a counted phase ahead.
+                // is ever two counted phases from the other.
                 bool ok = !on || wait_all(&ctl->q_full[i], q_n & 1u);
                 q_n += on;
                 // t < 0: the first two S. Then O(t) and the S that takes its P's place; the

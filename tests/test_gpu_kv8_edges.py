@@ -311,3 +311,17 @@ def test_windows_that_are_cut(nv, torch, dtype, window, sinks, seqs):
     b = Batch(nv, torch, seqs, 4, 1, 64, dtype=dtype, window=window, sinks=sinks, seed=sinks)
     b.call()
     b.check()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("ctx", [40, 900])
+def test_rows_of_zeros_alone_at_large_scores(nv, torch, dtype, ctx):
+    """All values 0 (exponent -100, the largest weights that there are) at scores near the
+    stated limit, rising by less than the step at which the reference moves."""
+    q, k, v = np.zeros((1, 1, 64)), np.zeros((ctx, 1, 64)), np.zeros((ctx, 1, 64))
+    q[:, :, 0], k[:, 0, 0] = 2.0 ** 20, 127.0
+    q[:, :, 1], k[:, 0, 1] = 1.0, np.linspace(0, 16, ctx)
+    v[-1] = 2.0 ** -60
+    Rows(nv, torch, q, k, v * 0, dtype, fmt="int8").check()
+    out = Rows(nv, torch, q, k, v, dtype, fmt="int8").out
+    assert torch.isfinite(out).all() and (out >= 0).all() and (out <= 2.0 ** -60).all()
